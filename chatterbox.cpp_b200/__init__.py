@@ -21,6 +21,7 @@ LIB_PATH = os.path.join(HERE, "libt3b200.so")
 
 T3B_OK = 0
 T3B_RNG_MT19937, T3B_RNG_PHILOX = 0, 1
+T3B_F32, T3B_F16, T3B_Q4_0, T3B_Q8_0, T3B_BF16 = 0, 1, 2, 8, 30   # ggml type ids
 ERRORS = {-1: "ARG", -2: "CUDA", -3: "OOM", -4: "STATE", -5: "DEVICE", -6: "CANCELLED", -7: "TIMEOUT"}
 
 # every symbol include/t3b200.h declares
@@ -31,6 +32,8 @@ EXPORTS = [
     "t3b_op_sample_philox", "t3b_expf_fixup_count", "t3b_op_expf", "t3b_op_attention_noalloc",
     "t3b_trace_hidden", "t3b_get_hidden_trace", "t3b_set_wait_limit", "t3b_launch_count", "t3b_s3gen_tokens",
     "t3b_op_check", "t3b_op_attention_prompt", "t3b_serve_submit", "t3b_serve_run", "t3b_serve_result", "t3b_serve_stats",
+    "t3b_op_kv_plan", "t3b_op_kv_append", "t3b_op_attention_shared", "t3b_op_attention_shared_prompt",
+    "t3b_op_attention_shared_workspace",
 ]
 
 
@@ -70,6 +73,37 @@ class Request(C.Structure):
     _fields_ = [("text", C.c_void_p), ("n_text", C.c_int32), ("cond_tokens", C.c_void_p), ("n_cond", C.c_int32),
                 ("spk_emb", C.c_void_p), ("params", SampleParams), ("rng_mode", C.c_int32), ("seed", C.c_uint64),
                 ("n_predict", C.c_int32), ("min_tokens", C.c_int32), ("max_retries", C.c_int32)]
+
+
+class PagedKv(C.Structure):
+    """t3b_paged_kv: one layer's pages of K and V."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("dtype", C.c_int32),
+                ("n_pages", C.c_int32), ("n_kv_head", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class KvPlan(C.Structure):
+    """t3b_kv_plan: a step's block tables, slots and positions."""
+    _fields_ = [("n", C.c_int32), ("page_size", C.c_int32), ("max_blocks", C.c_int32), ("rows_cap", C.c_int32),
+                ("len", C.c_void_p), ("add", C.c_void_p), ("release", C.c_void_p), ("free_pages", C.c_void_p),
+                ("free_cap", C.c_int32), ("n_free", C.c_void_p), ("n_free_out", C.c_void_p), ("table", C.c_void_p),
+                ("row_start", C.c_void_p), ("row_req", C.c_void_p), ("row_pos", C.c_void_p), ("slots", C.c_void_p),
+                ("len_out", C.c_void_p)]
+
+
+class KvAppend(C.Structure):
+    """t3b_kv_append: new K and V rows into their pages."""
+    _fields_ = [("cache", PagedKv), ("k", C.c_void_p), ("v", C.c_void_p), ("stride", C.c_int64), ("slots", C.c_void_p),
+                ("dtype", C.c_int32), ("rows", C.c_int32)]
+
+
+class SharedAttn(C.Structure):
+    """t3b_shared_attn: attention over shared prefixes and own pages."""
+    _fields_ = [("cache", PagedKv), ("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("len", C.c_void_p), ("table", C.c_void_p), ("row_start", C.c_void_p),
+                ("prefix_start", C.c_void_p), ("prefix_len", C.c_void_p), ("prefix_table", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("dtype", C.c_int32), ("n_head", C.c_int32),
+                ("n", C.c_int32), ("rows", C.c_int32), ("max_blocks", C.c_int32), ("n_prefix", C.c_int32),
+                ("prefix_max_blocks", C.c_int32), ("scale", C.c_float)]
 
 
 _lib = None
@@ -121,6 +155,11 @@ def lib():
             "t3b_serve_run": (C.c_int, [vp, C.c_int, i32p, i32p]),
             "t3b_serve_result": (C.c_int, [vp, C.c_int, vp, C.c_int, i32p, i32p]),
             "t3b_serve_stats": (C.c_int, [vp, C.POINTER(C.c_longlong), C.POINTER(C.c_double)]),
+            "t3b_op_kv_plan": (C.c_int, [C.POINTER(KvPlan), vp]),
+            "t3b_op_kv_append": (C.c_int, [C.POINTER(KvAppend), vp]),
+            "t3b_op_attention_shared": (C.c_int, [C.POINTER(SharedAttn), vp]),
+            "t3b_op_attention_shared_prompt": (C.c_int, [C.POINTER(SharedAttn), vp]),
+            "t3b_op_attention_shared_workspace": (C.c_size_t, [C.POINTER(SharedAttn)]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)

@@ -19,6 +19,8 @@
 #define T3B_DEVERR_TOKEN   1u   // token id outside the embedding table
 #define T3B_DEVERR_POS     2u   // position outside the KV cache / wpe table
 #define T3B_DEVERR_TIMEOUT 4u   // a bounded spin-wait gave up
+#define T3B_DEVERR_PAGE    8u   // page id or slot outside the paged cache
+#define T3B_DEVERR_FULL    16u  // too few free pages or rows for a step
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -1736,13 +1736,16 @@ extern "C" int t3b_op_attention_noalloc(const float * q_dev, const void * k_dev,
     return T3B_OK;
 }
 
+#include "paged.cuh"
+
 // Reads and clears the device error words of the op-level attention entry
-// points on the current device, after the stream's work so far.
+// points and of the paged operators on the current device, after the
+// stream's work so far.
 extern "C" int t3b_op_check(void * cuda_stream) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) { set_err(nullptr, "t3b_op_check: no device"); return T3B_ERR_CUDA; }
     cudaStream_t st = (cudaStream_t) cuda_stream;
-    unsigned * words[2] = {nullptr, nullptr};
+    unsigned * words[3] = {nullptr, nullptr, nullptr};
     {
         std::lock_guard<std::mutex> lk(g_op_mu);
         auto it = g_op.find(dev);
@@ -1752,6 +1755,10 @@ extern "C" int t3b_op_check(void * cuda_stream) {
         std::lock_guard<std::mutex> lk(g_noalloc_mu);
         auto it = g_noalloc.find(dev);
         if (it != g_noalloc.end()) words[1] = it->second.cnt + T3B_NOALLOC_CNT;
+    }
+    if (cudaGetSymbolAddress((void **) &words[2], g_paged_err) != cudaSuccess) {
+        set_err(nullptr, "t3b_op_check: cudaGetSymbolAddress failed");
+        return T3B_ERR_CUDA;
     }
     if (cudaStreamSynchronize(st) != cudaSuccess) { set_err(nullptr, "t3b_op_check: stream failed"); return T3B_ERR_CUDA; }
     unsigned w = 0;
@@ -1766,8 +1773,9 @@ extern "C" int t3b_op_check(void * cuda_stream) {
         w |= v;
     }
     if (w) {
-        set_err(nullptr, "op-level device check failed (error word 0x%x:%s%s)", w,
-                (w & T3B_DEVERR_POS) ? " length-out-of-range" : "", (w & T3B_DEVERR_TOKEN) ? " token-out-of-range" : "");
+        set_err(nullptr, "op-level device check failed (error word 0x%x:%s%s%s%s)", w,
+                (w & T3B_DEVERR_POS) ? " length-out-of-range" : "", (w & T3B_DEVERR_TOKEN) ? " token-out-of-range" : "",
+                (w & T3B_DEVERR_PAGE) ? " page-out-of-range" : "", (w & T3B_DEVERR_FULL) ? " out-of-pages-or-rows" : "");
         return T3B_ERR_DEVICE;
     }
     return T3B_OK;

@@ -47,7 +47,8 @@ extern "C" {
 #define T3B_ERR_TIMEOUT   -7   /* a bounded device-side wait ran out          */
 
 /* ggml type ids of the tensors the T3 GGUF holds */
-enum t3b_dtype { T3B_F32 = 0, T3B_F16 = 1, T3B_Q4_0 = 2, T3B_Q8_0 = 8 };
+enum t3b_dtype { T3B_F32 = 0, T3B_F16 = 1, T3B_Q4_0 = 2, T3B_Q8_0 = 8,
+                 T3B_BF16 = 30 /* only in the paged cache and its operators; no T3 GGUF tensor has it */ };
 
 /* One GGUF tensor view: name as written by convert-t3-turbo-to-gguf.py
  * (map_tensor_name, :147-194), ggml type, ggml shape (ne[0] contiguous),
@@ -319,8 +320,170 @@ int t3b_op_attention_noalloc(const float * q_dev, const void * k_dev, const void
                              int n_head, int max_ctx, const int32_t * len_dev, float * out_dev,
                              void * cuda_stream);
 
+/* ---------------- paged K/V cache with shared prefixes ------------------
+ * The dense caches above hold [n_head][max_ctx][64] per row, each with its
+ * own copy of the voice's conditioning, although the first 1 + n_cond keys
+ * and values are the same for every utterance of a voice and for both rows
+ * of a CFG stream (eval_prompt's row assembly, main.cpp:625-640).  These
+ * entry points keep K/V in pages of one pool instead: a prefix's pages are
+ * held once and its attention is computed for the whole batch at once, and
+ * each request's own tokens lie in pages that it takes from a stack of free
+ * ones.  They have no counterpart in chatterbox.cpp.
+ *
+ * One step of a serving loop: t3b_op_kv_plan (pages, slots and positions of
+ * the new tokens), then for each layer t3b_op_kv_append and
+ * t3b_op_attention_shared (one token per request) or
+ * t3b_op_attention_shared_prompt (several).  All of it runs on the caller's
+ * stream without a host synchronisation or an allocation, so a step can be
+ * captured into a CUDA graph; the structs are read during the call only.
+ * Pointers are device pointers of the current device unless noted.  Errors
+ * found on the device are kept for t3b_op_check. */
+
+/* One layer's pages: k and v are [n_pages][n_kv_head][page_size][head_dim],
+ * each page page_stride elements after the one before (0 = dense, i.e.
+ * n_kv_head * page_size * head_dim; larger strides let K and V, or several
+ * layers, share a page).  k and v are 16-byte aligned, page_stride a
+ * multiple of 8.  page_size is 8, 16, 32, 64, 128 or 256, head_dim 64 or
+ * 128, and n_pages * page_size fits 31 bits. */
+typedef struct t3b_paged_kv {
+    void *  k;
+    void *  v;
+    int64_t page_stride;
+    int32_t dtype;           /* T3B_F16 or T3B_BF16 */
+    int32_t n_pages;
+    int32_t n_kv_head;
+    int32_t page_size;
+    int32_t head_dim;
+} t3b_paged_kv;
+
+/* Block tables and slot maps of a step, from the requests' lengths.
+ *
+ * Request i holds len[i] own tokens in its first ceil(len / page_size)
+ * table entries and gets add[i] new ones (0 for an idle slot).  release[i]
+ * > 0 gives back the pages of the release[i] tokens that a finished request
+ * left in slot i first; its len[i] is then 0, and add[i] may already admit
+ * the next request.  free_pages is a stack of page ids with *n_free entries:
+ * released pages are pushed in request order, then new pages are popped in
+ * request order, k-th new page = stack[top - 1 - k], and written to
+ * table[i][ceil(len / page_size) ..].
+ *
+ * Row r of the step's row_start[n] rows is a new token of request row_req[r]
+ * at own position row_pos[r], stored at slot table[i][pos / page_size] *
+ * page_size + pos % page_size.  Rows from row_start[n] to rows_cap (which a
+ * captured graph may keep above what a step needs) get -1 in all three.
+ *
+ * n_free_out may be n_free and len_out may be len; otherwise no array may
+ * overlap another.  A step that does not fit (a negative length, more than
+ * max_blocks pages for a request, too few free pages, more than rows_cap
+ * rows, release[i] > 0 with len[i] > 0, n_free outside the stack, or no room
+ * on it) changes nothing: table and stack stay as they are, n_free_out =
+ * n_free, len_out = len, row_start is 0, all rows are -1, and t3b_op_check
+ * reports it.  n <= 8192. */
+typedef struct t3b_kv_plan {
+    int32_t n;               /* requests (slots) */
+    int32_t page_size;
+    int32_t max_blocks;      /* entries of a table row */
+    int32_t rows_cap;        /* entries of row_req, row_pos and slots */
+    const int32_t * len;     /* [n] own tokens before the step */
+    const int32_t * add;     /* [n] new tokens */
+    const int32_t * release; /* [n] tokens whose pages come back; NULL = none */
+    int32_t *       free_pages;   /* [free_cap] */
+    int32_t         free_cap;
+    const int32_t * n_free;       /* [1] */
+    int32_t *       n_free_out;   /* [1] */
+    int32_t *       table;        /* [n][max_blocks] */
+    int32_t *       row_start;    /* [n + 1] */
+    int32_t *       row_req;      /* [rows_cap], NULL = not wanted */
+    int32_t *       row_pos;      /* [rows_cap], NULL = not wanted */
+    int32_t *       slots;        /* [rows_cap], NULL = not wanted */
+    int32_t *       len_out;      /* [n] len + add, NULL = not wanted */
+} t3b_kv_plan;
+
+int t3b_op_kv_plan(const t3b_kv_plan * plan, void * cuda_stream);
+
+/* Writes rows of K and V, [rows][n_kv_head * head_dim] each `stride`
+ * elements after the one before, to their slots (ggml_cpy into memory_k /
+ * memory_v, main.cpp:528-540).  Rows whose slot is negative are skipped; a
+ * slot past the last page is skipped and reported.  dtype T3B_F32 (rounded
+ * to the cache's type) or the cache's own; F32 rows go into an F16 or a BF16
+ * cache.  k, v and the stride are multiples of 16 bytes.  Slots of one call
+ * are distinct. */
+typedef struct t3b_kv_append {
+    t3b_paged_kv    cache;
+    const void *    k;
+    const void *    v;
+    int64_t         stride;
+    const int32_t * slots;   /* [rows] */
+    int32_t         dtype;
+    int32_t         rows;
+} t3b_kv_append;
+
+int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
+
+/* Attention of a batch over shared prefixes and own pages.
+ *
+ * Requests prefix_start[p] .. prefix_start[p + 1] - 1 see the prefix_len[p]
+ * keys in the pages of prefix_table[p] and then their own: key j of request
+ * i is row j % page_size of page table[i][j / page_size].  Requests outside
+ * every range have no prefix; n_prefix 0 needs no prefix pointers.  Table
+ * entries past a length are not read.  Query head h reads K/V head h *
+ * n_kv_head / n_head.  out = softmax(scale * q.K) V, rounded once.
+ *
+ *   t3b_op_attention_shared: q and out have one row per request (rows = n,
+ *   row_start unused); row i sees its prefix and own keys 0 .. len[i] - 1.
+ *   t3b_op_attention_shared_prompt: request i has rows row_start[i] ..
+ *   row_start[i + 1] - 1, its last add_i own tokens: row r sees the prefix
+ *   and own keys 0 .. len[i] - add_i + r - row_start[i].  len is the length
+ *   AFTER the append.  rows bounds row_start[n]; rows of out from
+ *   row_start[n] on stay as they were.
+ *
+ * A row with no key at all is zero.  A request whose length is negative or
+ * past its table, or whose rows exceed its length, and a prefix length past
+ * its table leave their rows unwritten and are reported; a page id outside
+ * the pool is reported and its keys count as absent.
+ *
+ * Types: q and out F32 with an F16 cache (scores, softmax and sums keep 22
+ * bits or more of every factor), or q, out and cache all F16 or all BF16
+ * (probabilities are rounded to that type before they meet V, which is less
+ * than the output's own rounding; sums stay in F32).  n_head is a multiple
+ * of n_kv_head, at most 16 times it.  scale 0 = 1 / sqrt(head_dim).  q, out
+ * and their strides are multiples of 16 bytes.  out may be q (with the same
+ * stride).  workspace holds t3b_op_attention_shared_workspace() bytes, 16-byte
+ * aligned; calls that can run at the same time need one each.  n and
+ * n_prefix <= 65535. */
+typedef struct t3b_shared_attn {
+    t3b_paged_kv    cache;
+    const void *    q;
+    void *          out;
+    int64_t         q_stride;      /* elements from row to row */
+    int64_t         out_stride;
+    const int32_t * len;           /* [n] */
+    const int32_t * table;         /* [n][max_blocks] */
+    const int32_t * row_start;     /* [n + 1], prompt form only */
+    const int32_t * prefix_start;  /* [n_prefix + 1] */
+    const int32_t * prefix_len;    /* [n_prefix] */
+    const int32_t * prefix_table;  /* [n_prefix][prefix_max_blocks] */
+    void *          workspace;
+    size_t          workspace_bytes;
+    int32_t         dtype;         /* of q and out */
+    int32_t         n_head;
+    int32_t         n;
+    int32_t         rows;
+    int32_t         max_blocks;
+    int32_t         n_prefix;
+    int32_t         prefix_max_blocks;
+    float           scale;
+} t3b_shared_attn;
+
+int t3b_op_attention_shared(const t3b_shared_attn * a, void * cuda_stream);
+int t3b_op_attention_shared_prompt(const t3b_shared_attn * a, void * cuda_stream);
+/* Bytes of workspace that either call needs for these sizes (pointers are
+ * not looked at); 0 for sizes that the calls refuse. */
+size_t t3b_op_attention_shared_workspace(const t3b_shared_attn * a);
+
 /* Synchronises cuda_stream, then reads and clears the device error words of
- * t3b_op_attention and t3b_op_attention_noalloc on the current device: a row
+ * t3b_op_attention, t3b_op_attention_noalloc and the paged operators on the
+ * current device: a row
  * whose len is <= 0 or > max_ctx is skipped by the kernel (its output left
  * unwritten) and reported here as T3B_ERR_DEVICE.  Errors stay recorded
  * until this call. */

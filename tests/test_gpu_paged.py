@@ -1,0 +1,538 @@
+"""GPU tests of the paged operators (t3b_op_kv_plan, t3b_op_kv_append,
+t3b_op_attention_shared, t3b_op_attention_shared_prompt) against plain
+references in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import paged_ref
+from paged_ref import Batch, blocks
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.init()
+
+
+@pytest.fixture(autouse=True)
+def _clean(pkg):
+    """No error is left over from another test, and none is left behind."""
+    pkg.lib().t3b_op_check(_stream())
+    yield
+    assert pkg.lib().t3b_op_check(_stream()) == 0, pkg.last_error()
+
+
+def _stream():
+    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _i32(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+# --------------------------------------------------------------------------
+# plan
+# --------------------------------------------------------------------------
+
+class Plan:
+    """The device arrays of a t3b_kv_plan, with a guard value behind each."""
+
+    def __init__(self, pkg, ln, add, release, page, table, free, n_free, rows_cap, in_place=False, want=True):
+        self.n, self.width = table.shape
+        self.in_ = dict(len=_i32(ln), add=_i32(add), table=_i32(np.r_[table.ravel(), 77]), free=_i32(np.r_[free, 77]), n_free=_i32([n_free]))
+        self.release = None if release is None else _i32(release)
+        self.out = {k: torch.full((m + 1,), 77, dtype=torch.int32, device="cuda")
+                    for k, m in (("row_start", self.n + 1), ("row_req", rows_cap), ("row_pos", rows_cap), ("slots", rows_cap),
+                                 ("len_out", self.n), ("n_free_out", 1))}
+        self.in_place = in_place
+        if in_place:
+            self.out["len_out"], self.out["n_free_out"] = self.in_["len"], self.in_["n_free"]
+        p = lambda t: t.data_ptr()  # noqa: E731
+        self.d = pkg.KvPlan(n=self.n, page_size=page, max_blocks=self.width, rows_cap=rows_cap, len=p(self.in_["len"]),
+                            add=p(self.in_["add"]), release=None if release is None else p(self.release),
+                            free_pages=p(self.in_["free"]), free_cap=len(free), n_free=p(self.in_["n_free"]),
+                            n_free_out=p(self.out["n_free_out"]), table=p(self.in_["table"]), row_start=p(self.out["row_start"]))
+        if want:
+            self.d.row_req, self.d.row_pos = p(self.out["row_req"]), p(self.out["row_pos"])
+            self.d.slots, self.d.len_out = p(self.out["slots"]), p(self.out["len_out"])
+
+    def got(self):
+        o = {k: v.cpu().numpy().astype(np.int64) for k, v in self.out.items()}
+        whole = ("len_out", "n_free_out") if self.in_place else ()
+        for k in o:
+            assert k in whole or o[k][-1] == 77, k                 # nothing is written past an array
+        r = {k: o[k] if k in whole else o[k][:-1] for k in o}
+        t, f = (self.in_[k].cpu().numpy().astype(np.int64) for k in ("table", "free"))
+        assert t[-1] == 77 and f[-1] == 77
+        return dict(r, table=t[:-1].reshape(self.n, self.width), free=f[:-1], n_free=int(r["n_free_out"][0]))
+
+
+def _same(got, ref):
+    for k, v in ref.items():
+        assert np.array_equal(np.asarray(got[k]), np.asarray(v)), k
+
+
+def _random_step(rng, n, page, width, readmit):
+    total = n * width
+    ids = rng.permutation(total)
+    used = rng.integers(0, width * page // 2, n)
+    kind = rng.integers(0, 4, n)                                   # decode, prompt, idle, finished
+    ln = np.where(kind == 1, 0, used)
+    release = np.where(kind == 3, used, 0)
+    ln = np.where(release > 0, 0, ln)
+    add = np.select([kind == 0, kind == 1], [np.ones(n, int), rng.integers(0, width * page + 1, n)], 0)
+    if readmit:
+        add = np.where(release > 0, rng.integers(0, width * page + 1, n), add)
+    add = np.minimum(add, width * page - ln)
+    table, at = np.full((n, width), -1), 0
+    for i in range(n):
+        b = blocks(ln[i] if release[i] == 0 else release[i], page)
+        table[i, :b] = ids[at:at + b]
+        at += b
+    free = np.r_[ids[at:], np.full(at, -5)]
+    return ln, add, release, table, free, total - at
+
+
+@pytest.mark.parametrize("n,page,width", [(1, 8, 1), (1, 256, 3), (2, 16, 4), (31, 8, 5), (64, 16, 40), (1000, 32, 6),
+                                          (1024, 8, 3), (1025, 64, 4), (8192, 16, 3)])
+@pytest.mark.parametrize("readmit", [False, True])
+def test_plan_matches_its_definition(pkg, n, page, width, readmit):
+    rng = np.random.default_rng(n + page)
+    for trial in range(3):
+        ln, add, release, table, free, n_free = _random_step(rng, n, page, width, readmit)
+        cap = int(add.sum()) + [0, 1, 700][trial]
+        p = Plan(pkg, ln, add, release, page, table, free, n_free, cap, in_place=trial == 1)
+        pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+        ref = paged_ref.plan(ln, add, release, page, table, free, n_free, cap)
+        assert ref is not None
+        _same(p.got(), ref)
+
+
+def test_plan_without_the_optional_arrays(pkg):
+    rng = np.random.default_rng(5)
+    ln, add, _, table, free, n_free = _random_step(rng, 40, 16, 6, False)
+    p = Plan(pkg, ln, add, None, 16, table, free, n_free, int(add.sum()), want=False)
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    ref = paged_ref.plan(ln, add, None, 16, table, free, n_free, int(add.sum()))
+    got = p.got()
+    _same({k: got[k] for k in ("table", "free", "n_free", "row_start")},
+          {k: ref[k] for k in ("table", "free", "n_free", "row_start")})
+    assert (got["row_req"] == 77).all() and (got["len_out"] == 77).all()
+
+
+BAD_STEPS = {
+    "negative length": dict(len={3: -1}), "negative new": dict(add={0: -2}), "negative release": dict(release={2: -7}),
+    "past the table": dict(add={1: 97}), "far past the table": dict(add={1: 2 ** 31 - 1}), "release past the table": dict(release={2: 97}, len={2: 0}),
+    "release of a live slot": dict(release={3: 5}), "too few pages": dict(n_free=2), "too few rows": dict(rows=19),
+    "stack below zero": dict(n_free=-1), "stack past its end": dict(n_free=1000),
+    "no room for returned pages": dict(free_cap=29, release={2: 90}, len={2: 0}, add={2: 0}),
+}
+
+
+@pytest.mark.parametrize("bad", list(BAD_STEPS), ids=str)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_step_that_does_not_fit_changes_nothing(pkg, bad, in_place):
+    n, page, width = 5, 16, 6
+    ln, add, release = np.array([0, 16, 0, 5, 33]), np.array([17, 1, 0, 1, 1]), np.zeros(5, int)
+    what = BAD_STEPS[bad]
+    for name, arr in (("len", ln), ("add", add), ("release", release)):
+        for i, v in what.get(name, {}).items():
+            arr[i] = v
+    table = np.full((n, width), -1)
+    table[1, :1], table[2], table[3, :1], table[4, :3] = 40, np.arange(50, 56), 41, [42, 43, 44]
+    free = np.arange(30)
+    p = Plan(pkg, ln, add, release, page, table, free[:what.get("free_cap", 30)], what.get("n_free", 28), what.get("rows", 40), in_place)
+    assert paged_ref.plan(ln, add, release, page, table, free[:what.get("free_cap", 30)], what.get("n_free", 28), what.get("rows", 40)) is None
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    assert pkg.lib().t3b_op_check(_stream()) == -5
+    assert "range" in pkg.last_error() or "out-of-pages" in pkg.last_error()
+    got = p.got()
+    _same({k: got[k] for k in ("table", "free", "n_free")}, dict(table=table, free=free[:what.get("free_cap", 30)], n_free=what.get("n_free", 28)))
+    assert (got["row_start"] == 0).all() and np.array_equal(got["len_out"], ln)
+    assert all((got[k] == -1).all() for k in ("row_req", "row_pos", "slots"))
+
+
+def test_captured_plan_evolves_its_state(pkg):
+    """A captured step with in-place lengths and stack, replayed: each replay
+    is the next step; pages run out at the right one."""
+    n, page, width = 33, 8, 4
+    ln, add = np.arange(n) % 5, np.ones(n, int)
+    table, free = np.full((n, width), -1), np.arange(70)[::-1].copy()
+    table[ln > 0, 0] = 100 + np.arange(n)[ln > 0]
+    p = Plan(pkg, ln, add, None, page, table, free, 70, 64, in_place=True)
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    state = dict(len_out=ln, table=table, free=free, n_free=70)
+    for step in range(25):
+        ref = paged_ref.plan(state["len_out"], add, None, page, state["table"], state["free"], state["n_free"], 64)
+        g.replay()
+        torch.cuda.synchronize()
+        if ref is None:
+            assert pkg.lib().t3b_op_check(_stream()) == -5
+            break
+        _same(p.got(), ref)
+        state = ref
+    assert step > 10 and ref is None
+
+
+# --------------------------------------------------------------------------
+# append
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("src,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("rows,kv,dim,page,pad,gap", [(1, 1, 64, 8, 0, 0), (5, 16, 64, 16, 0, 0), (333, 3, 128, 32, 24, 8),
+                                                      (2049, 8, 128, 64, 0, 8 * 64 * 128), (64, 2, 64, 256, 8, 0)])
+def test_append_matches_its_definition(pkg, src, cache, rows, kv, dim, page, pad, gap):
+    t = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+    ids = {"f32": 0, "f16": 1, "bf16": 30}
+    g = torch.Generator().manual_seed(rows)
+    n_pages = blocks(rows, page) + 3
+    stride = kv * page * dim + gap
+    pool = torch.randn(2, n_pages * stride, generator=g).to(t[cache]).cuda()
+    before = pool.clone()
+    new = (torch.randn(2, rows, kv * dim + pad, generator=g) * 50).to(t[src]).cuda()
+    if src == "f32":
+        new[0, 0, :4] = torch.tensor([7e4, -1e30, float("inf"), float("nan")])   # past f16, and not finite
+    slots = torch.randperm(n_pages * page, generator=g)[:rows].to(torch.int32)
+    if rows > 4:
+        slots[1::5] = -1
+    sd = slots.cuda()
+    c = pkg.PagedKv(k=pool[0].data_ptr(), v=pool[1].data_ptr(), page_stride=stride, dtype=ids[cache], n_pages=n_pages,
+                    n_kv_head=kv, page_size=page, head_dim=dim)
+    a = pkg.KvAppend(cache=c, k=new[0].data_ptr(), v=new[1].data_ptr(), stride=kv * dim + pad, slots=sd.data_ptr(),
+                     dtype=ids[src], rows=rows)
+    pkg.check(pkg.lib().t3b_op_kv_append(C.byref(a), _stream()))
+    for x in range(2):
+        want = before[x].cpu().clone()
+        view = want.view(n_pages, stride)[:, :kv * page * dim].view(n_pages, kv, page, dim)
+        for r in range(rows):
+            s = int(slots[r])
+            if s >= 0:
+                view[s // page, :, s % page] = new[x, r, :kv * dim].cpu().to(t[cache]).view(kv, dim)
+        assert torch.equal(pool[x].cpu().view(torch.int16), want.view(torch.int16)) or \
+            torch.allclose(pool[x].cpu(), want, rtol=0, atol=0, equal_nan=True)
+
+
+def test_append_reports_a_slot_past_the_pool(pkg):
+    pool = torch.zeros(2, 4 * 16 * 64, dtype=torch.float16, device="cuda")
+    new = torch.ones(2, 3, 64, device="cuda")
+    slots = _i32([3, 64, 2 ** 31 - 1])
+    c = pkg.PagedKv(k=pool[0].data_ptr(), v=pool[1].data_ptr(), dtype=1, n_pages=4, n_kv_head=1, page_size=16, head_dim=64)
+    a = pkg.KvAppend(cache=c, k=new[0].data_ptr(), v=new[1].data_ptr(), stride=64, slots=slots.data_ptr(), dtype=0, rows=3)
+    pkg.check(pkg.lib().t3b_op_kv_append(C.byref(a), _stream()))
+    assert pkg.lib().t3b_op_check(_stream()) == -5
+    assert "page-out-of-range" in pkg.last_error()
+    assert float(pool.sum()) == 2 * 64
+
+
+# --------------------------------------------------------------------------
+# attention
+# --------------------------------------------------------------------------
+
+def _attend(pkg, b, **kw):
+    d = b.desc(pkg, **kw)
+    f = pkg.lib().t3b_op_attention_shared if b.adds is None else pkg.lib().t3b_op_attention_shared_prompt
+    pkg.check(f(C.byref(d), _stream()))
+    torch.cuda.synchronize()
+    return d
+
+
+def _close(b, out=None, scale=None, skip=()):
+    ref, tol = b.reference(scale)
+    w = b.heads * b.dim
+    got = (b.out_all if out is None else out)[:b.rows, :w].cpu().double()
+    keep = torch.ones(b.rows, dtype=torch.bool)
+    for i in skip:
+        keep[b.starts[i]:b.starts[i + 1]] = False
+    got, ref, tol = got[keep], ref[keep], tol[keep]
+    assert torch.isfinite(got).all()
+    over = (got - ref).abs() / tol
+    assert over.max() <= 1, (float(over.max()), int(over.argmax()))
+    if b.kind == "f32" and ref.numel() and ref.norm() > 0:
+        # errors of 22-bit factors and 32-bit sums do not add up in one direction
+        assert (got - ref).norm() / ref.norm() < 3e-6
+    # rows behind the last one and the padding of each row stay as they were
+    if out is None:
+        assert (b.out_all[b.rows:] == -7).all() and (b.out_all[:b.rows, w:] == -7).all()
+
+
+LAYOUTS = [(1, 1, 64, 16), (4, 4, 64, 8), (16, 16, 64, 16), (8, 2, 128, 32), (6, 2, 64, 64), (16, 1, 128, 128),
+           (7, 1, 64, 256), (5, 5, 128, 16), (10, 2, 128, 64), (24, 2, 64, 32)]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page", LAYOUTS)
+def test_decode_attention_matches_fp64(pkg, kind, heads, kv, dim, page):
+    lens = [1, 0, page - 1, page, page + 1, 2 * page + 3, 63, 64, 65, 300, 129]
+    for prefix, start in (([], None), ([1], [0, 11]), ([page + 3, 0, 200], [1, 4, 6, 10]), ([64, 128], [0, 1, 11])):
+        b = Batch(kind, lens, heads, kv, dim, page, prefix, start, seed=heads * 7 + len(prefix), gap=8 * len(prefix), q_pad=8 * len(prefix))
+        _attend(pkg, b)
+        _close(b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,heads,kv,dim,page,prefix,lo,hi", [
+    (1, 16, 16, 64, 16, 376, 1, 1), (2, 16, 16, 64, 16, 376, 88, 1088), (3, 4, 4, 64, 16, 1, 1500, 1501), (1, 8, 8, 128, 64, 0, 5000, 5001),
+    (130, 4, 2, 64, 16, 77, 1, 40), (65, 32, 8, 128, 32, 1000, 1, 90), (300, 2, 1, 64, 8, 513, 0, 30), (1, 1, 1, 128, 16, 4000, 0, 1)])
+def test_decode_attention_sizes(pkg, kind, n, heads, kv, dim, page, prefix, lo, hi):
+    rng = np.random.default_rng(n + heads)
+    b = Batch(kind, rng.integers(lo, hi + 1, n).tolist(), heads, kv, dim, page, [prefix], [0, n], seed=n)
+    _attend(pkg, b)
+    _close(b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim,page", LAYOUTS)
+def test_prompt_attention_matches_fp64_ragged(pkg, kind, heads, kv, dim, page):
+    adds = [1, 0, page, 33, 5, 0, 130, 64]
+    lens = [1, 0, page, 50, 5 + page, 7, 130, 300]
+    for prefix, start in (([], None), ([page + 3, 0, 200], [0, 2, 3, 7]), ([65], [0, 8])):
+        b = Batch(kind, lens, heads, kv, dim, page, prefix, start, adds=adds, seed=heads * 3 + len(prefix), gap=8, q_pad=16)
+        _attend(pkg, b)
+        _close(b)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("adds,past,heads,kv,dim,page,prefix", [
+    ([88, 120, 20], [0, 0, 0], 16, 16, 64, 16, 376), ([700, 1], [333, 2000], 4, 2, 128, 64, 129), ([1000], [0], 2, 1, 64, 32, 0),
+    ([3], [4000], 8, 8, 64, 16, 500), ([1] * 150, [7] * 150, 4, 1, 128, 16, 40), ([257, 256, 255], [1, 0, 127], 3, 3, 128, 128, 1)])
+def test_prompt_attention_sizes(pkg, kind, adds, past, heads, kv, dim, page, prefix):
+    b = Batch(kind, [a + p for a, p in zip(adds, past)], heads, kv, dim, page, [prefix], [0, len(adds)], adds=adds, seed=adds[0])
+    _attend(pkg, b)
+    _close(b)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("kind,q_scale", [("f32", 3e4), ("f32", 1e-6), ("f16", 100.0), ("bf16", 300.0), ("f32", 0.0)])
+def test_large_and_small_queries(pkg, kind, q_scale, prompt):
+    """Scores of thousands (the softmax picks one key) and of nothing (it averages)."""
+    lens = [40, 200, 1]
+    b = Batch(kind, lens, 4, 2, 64, 16, [100], [0, 3], adds=[40, 30, 1] if prompt else None, seed=3, q_scale=q_scale)
+    _attend(pkg, b)
+    ref, tol = b.reference()
+    got = b.out_all[:b.rows].cpu().double()
+    assert torch.isfinite(got).all()
+    assert ((got - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("scale", [0.3, -0.125])
+def test_scale_argument(pkg, prompt, scale):
+    b = Batch("f32", [40, 100], 4, 2, 64, 16, [50], [0, 2], adds=[40, 30] if prompt else None, seed=4)
+    d = b.desc(pkg)
+    d.scale = scale
+    f = pkg.lib().t3b_op_attention_shared_prompt if prompt else pkg.lib().t3b_op_attention_shared
+    pkg.check(f(C.byref(d), _stream()))
+    torch.cuda.synchronize()
+    _close(b, scale=scale)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_output_in_place_of_q(pkg, prompt, kind):
+    b = Batch(kind, [40, 3, 700], 8, 4, 64, 16, [300], [0, 3], adds=[40, 2, 300] if prompt else None, seed=5)
+    out = b.q_all.clone()
+    b.q_all, b.q = out, out[:, :8 * 64]
+    ref, tol = b.reference()
+    _attend(pkg, b, out=out)
+    assert ((out.cpu().double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_bad_lengths_and_pages_are_reported(pkg, prompt):
+    """A request with a bad length leaves its rows unwritten, a bad page's
+    keys count as absent, and the other requests are right."""
+    lens, adds = [40, 30, 20, 50], [3, 30, 2, 1]
+    for what in ("long", "negative", "page", "prefix"):
+        b = Batch("f32", lens, 4, 2, 64, 16, [20, 20], [0, 2, 4], adds=adds if prompt else None, seed=6)
+        skip = [1]
+        if what == "long":
+            b.len[1] = b.table.shape[1] * 16 + 1
+        elif what == "negative":
+            b.len[1] = -3
+        elif what == "prefix":
+            b.plen[0], skip = 100, [0, 1]
+        else:
+            b.table[1, 0] = [b.n_pages, -1][prompt]
+        _attend(pkg, b)
+        assert pkg.lib().t3b_op_check(_stream()) == -5
+        assert ("page-out-of-range" if what == "page" else "length-out-of-range") in pkg.last_error()
+        _close(b, skip=skip)
+        rows = b.out_all[b.starts[1]:b.starts[2]]
+        if what == "page":                                        # the other 14 own keys and the prefix are left
+            b.own[1] = b.own[1][:, 16:]
+            if not prompt:
+                _close(b)
+        else:
+            assert (rows == -7).all()
+
+
+def test_more_rows_than_keys_are_reported(pkg):
+    b = Batch("f32", [4, 9], 4, 2, 64, 16, [20], [0, 2], adds=[4, 9], seed=6)
+    b.len[0] = 3
+    _attend(pkg, b)
+    assert pkg.lib().t3b_op_check(_stream()) == -5
+    _close(b, skip=[0])
+    assert (b.out_all[:4] == -7).all()
+
+
+def test_a_workspace_of_another_call_leaves_no_trace(pkg):
+    """Two batches through one workspace, one after the other and back."""
+    x = Batch("f32", [40] * 20, 4, 4, 64, 16, [300], [0, 20], seed=7)
+    y = Batch("f32", [3, 500], 4, 4, 64, 16, [20, 700], [0, 1, 2], seed=8)
+    dx, dy = x.desc(pkg), y.desc(pkg)
+    big = torch.empty(max(dx.workspace_bytes, dy.workspace_bytes, 16), dtype=torch.uint8, device="cuda").fill_(0xFF)
+    for b, d in ((x, dx), (y, dy), (x, dx)):
+        d.workspace, d.workspace_bytes = big.data_ptr(), big.numel()
+        b.out_all.fill_(-7)
+        pkg.check(pkg.lib().t3b_op_attention_shared(C.byref(d), _stream()))
+        torch.cuda.synchronize()
+        _close(b)
+
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_repeated_calls_give_the_same_bits(pkg, prompt):
+    b = Batch("f32", [40, 900, 7, 333], 8, 8, 64, 16, [377], [0, 4], adds=[40, 60, 7, 100] if prompt else None, seed=9)
+    _attend(pkg, b)
+    first = b.out_all.clone()
+    for _ in range(5):
+        _attend(pkg, b)
+        assert torch.equal(b.out_all, first)
+
+
+def test_two_calls_at_once_on_two_streams(pkg):
+    bs = [Batch("f32", [200, 30, 77] * 8, 8, 8, 64, 16, [377], [0, 24], seed=10 + i) for i in range(2)]
+    ds = [b.desc(pkg) for b in bs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for d, s in zip(ds, streams):
+            pkg.check(pkg.lib().t3b_op_attention_shared(C.byref(d), C.c_void_p(s.cuda_stream)))
+    torch.cuda.synchronize()
+    for b in bs:
+        _close(b)
+
+
+@pytest.mark.parametrize("dim,prompt", [(64, False), (128, True)])
+def test_pages_past_2_to_the_31_elements(pkg, dim, prompt):
+    """Page offsets that do not fit 32 bits: K and V of 4.4 GB each."""
+    page, kv = 64, 8
+    at = (1 << 31) // (page * kv * dim) + 3
+    b = Batch("f16", [70, 200], 8, kv, dim, page, [100], [0, 2], adds=[70, 10] if prompt else None, seed=11, pages_at=at)
+    assert b.k.numel() > 1 << 31
+    _attend(pkg, b)
+    _close(b)
+
+
+# --------------------------------------------------------------------------
+# the operators together
+# --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_serving_loop_matches_dense_attention(pkg, graph):
+    """Plan, append and attention as a server runs them: prompts of a common
+    prefix are admitted, decode, finish, and their slots are taken over by
+    others; every step's output equals t3b_op_attention on dense caches that
+    hold prefix and own keys of each request.  With `graph` each kind of step
+    is captured once and replayed."""
+    L = pkg.lib()
+    H, D, page, n, width, cap, P = 16, 64, 16, 6, 7, 64, 37
+    rng = np.random.default_rng(12)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n_pages = 40
+    pool = torch.full((2, n_pages, H, page, D), float("nan"), dtype=torch.float16, device="cuda")
+    pre_pages = blocks(P, page)
+    dense = torch.zeros(2, n, H, 256, D, dtype=torch.float16, device="cuda")
+    kvp = torch.randn(2, P, H, D, generator=g, device="cuda").half()
+    ptable = torch.arange(pre_pages, dtype=torch.int32, device="cuda")
+    for t in range(P):
+        pool[:, t // page, :, t % page] = kvp[:, t]
+    dense[:, :, :, :P] = kvp.permute(0, 2, 1, 3)[:, None]
+    st = torch.cuda.Stream()
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    ln, add, rel, table = z(n), z(n), z(n), z(n, width)
+    free, n_free = torch.arange(pre_pages, n_pages, dtype=torch.int32, device="cuda"), _i32([n_pages - pre_pages])
+    row_start, req, pos, slots = z(n + 1), z(cap), z(cap), z(cap)
+    plen, pstart = _i32([P]), _i32([0, n])
+    q, k, v, out = (torch.zeros(cap, H * D, device="cuda") for _ in range(4))
+    p = lambda t: t.data_ptr()  # noqa: E731
+    dplan = pkg.KvPlan(n=n, page_size=page, max_blocks=width, rows_cap=cap, len=p(ln), add=p(add), release=p(rel), free_pages=p(free),
+                       free_cap=free.numel(), n_free=p(n_free), n_free_out=p(n_free), table=p(table), row_start=p(row_start),
+                       row_req=p(req), row_pos=p(pos), slots=p(slots), len_out=p(ln))
+    cache = pkg.PagedKv(k=p(pool[0]), v=p(pool[1]), dtype=1, n_pages=n_pages, n_kv_head=H, page_size=page, head_dim=D)
+    dapp = pkg.KvAppend(cache=cache, k=p(k), v=p(v), stride=H * D, slots=p(slots), dtype=0, rows=cap)
+    da = pkg.SharedAttn(cache=cache, q=p(q), out=p(out), q_stride=H * D, out_stride=H * D, len=p(ln), table=p(table),
+                        row_start=p(row_start), prefix_start=p(pstart), prefix_len=p(plen), prefix_table=p(ptable), dtype=0,
+                        n_head=H, n=n, rows=cap, max_blocks=width, n_prefix=1, prefix_max_blocks=pre_pages)
+    dd = pkg.SharedAttn.from_buffer_copy(da)
+    dd.rows, dd.row_start = n, None
+    size = max(L.t3b_op_attention_shared_workspace(C.byref(da)), L.t3b_op_attention_shared_workspace(C.byref(dd)))
+    ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+    for d in (da, dd):
+        d.workspace, d.workspace_bytes = p(ws), ws.numel()
+
+    def step(decode):
+        s = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        pkg.check(L.t3b_op_kv_plan(C.byref(dplan), s))
+        pkg.check(L.t3b_op_kv_append(C.byref(dapp), s))
+        if decode:
+            pkg.check(L.t3b_op_attention_shared(C.byref(dd), s))
+        else:
+            pkg.check(L.t3b_op_attention_shared_prompt(C.byref(da), s))
+
+    graphs = {}
+    if graph:
+        for decode in (False, True):
+            graphs[decode] = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graphs[decode], stream=st):
+                step(decode)
+    lens, live = np.zeros(n, int), np.zeros(n, bool)
+    for it in range(24):
+        decode = it % 3 != 0
+        a, r = np.zeros(n, int), np.zeros(n, int)
+        if decode:
+            a[:] = 1                                   # one row per request: every slot gets a token
+        else:
+            gone = live & (rng.random(n) < 0.5)
+            r[gone], lens[gone] = lens[gone], 0
+            a = np.where(lens == 0, rng.integers(1, 10, n), 1)
+        a = np.minimum(a, width * page - lens)
+        live[:] = True
+        add.copy_(_i32(a)); rel.copy_(_i32(r))
+        if r.any():
+            ln.copy_(_i32(lens))
+        x = torch.randn(3, cap, H * D, generator=g, device="cuda")
+        q.copy_(x[0]); k.copy_(x[1]); v.copy_(x[2]); out.fill_(-7.0)
+        torch.cuda.synchronize()
+        if graph:
+            graphs[decode].replay()
+        else:
+            step(decode)
+        torch.cuda.synchronize()
+        pkg.check(L.t3b_op_check(_stream()))
+        starts = np.cumsum(np.r_[0, a])
+        total = int(starts[-1])
+        assert row_start.tolist() == starts.tolist() and ln.tolist() == (lens + a).tolist()
+        rows, rlen = [], []
+        for i in range(n):
+            for t in range(a[i]):
+                dense[0, i, :, P + lens[i] + t] = k[starts[i] + t].half().view(H, D)
+                dense[1, i, :, P + lens[i] + t] = v[starts[i] + t].half().view(H, D)
+                rows.append(i)
+                rlen.append(P + lens[i] + t + 1)
+        kd, vd = dense[0][rows].contiguous(), dense[1][rows].contiguous()
+        want = torch.zeros(total, H * D, device="cuda")
+        pkg.check(L.t3b_op_attention(p(q), p(kd), p(vd), total, H, 256, p(_i32(rlen)), p(want), _stream()))
+        torch.cuda.synchronize()
+        assert (out[:total] - want).abs().max() <= 1e-5 * want.abs().max()     # the bound of each against 64 bits
+        assert (out[total:] == -7).all()
+        lens = lens + a
