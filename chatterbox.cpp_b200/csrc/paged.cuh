@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <type_traits>
 
 // Error word of the paged operators on each device (read and cleared by
 // t3b_op_check).  Kernels name it directly, so a launch needs no address
@@ -290,6 +291,364 @@ __global__ __launch_bounds__(128) void attn_shared_simple_kernel(PgAttn a) {
     }
 }
 
+// ---- decode: one query token per request -----------------------------------
+//
+// Bound by HBM: each own key and value is read once and meets group (1 to 16)
+// queries.  One CTA (or a cluster of them, each with a range of the keys) per
+// (request, kv head); its four warps take 16-key tiles in turn, each with its
+// own ring of cp.async stages, so no barrier stands between a tile's arrival
+// and its use.  The arithmetic is mma.sync m16n8k16 with the group's queries
+// as the 16 rows (there are too few of them for a 128-row tcgen05 tile):
+// S = Q K^T comes out in the layout in which P enters P V, so the softmax
+// stays in registers.  F32 queries take two rows, hi and lo, of 11 bits each
+// (K and V are exact in f16), and so do their probabilities.
+#define PD_WARPS 4
+#define PD_TK 16                // keys of a tile
+#define PD_LAZY 8.0f            // a row is rescaled when its maximum grew by 2^8 or more
+
+template <class CT> struct PgBias { static constexpr float v = 0.0f; };
+// f16 probabilities are held times 2^7: with the lazy maximum they stay below 2^15, and what
+// falls under f16's normal range is 2^-21 of the largest or less
+template <> struct PgBias<__half> { static constexpr float v = 7.0f; };
+
+__device__ __forceinline__ float pg_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void pg_cp16(unsigned dst, const void * src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void pg_ldm4(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pg_ldm4t(unsigned (&r)[4], unsigned addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <class CT>
+__device__ __forceinline__ void pg_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    if (std::is_same<CT, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// two floats as a pair of the cache's type, the first in the low half
+template <class CT> __device__ __forceinline__ unsigned pg_pack2(float x, float y);
+template <> __device__ __forceinline__ unsigned pg_pack2<__half>(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const unsigned *) &h;
+}
+template <> __device__ __forceinline__ unsigned pg_pack2<__nv_bfloat16>(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const unsigned *) &h;
+}
+// x and y as hi + lo pairs of f16: hi is x rounded, lo what that lost
+__device__ __forceinline__ void pg_split2(float x, float y, unsigned & hi, unsigned & lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *(const unsigned *) &h;
+    lo = *(const unsigned *) &l;
+}
+// The power of two by which an F32 query row is divided before it is split:
+// it brings the row's largest element to [2^8, 2^9), so that neither part
+// leaves f16's range.  Zero and non-finite rows keep their values.
+__device__ __forceinline__ int pg_row_exp(float mx) {
+    if (!(mx > 0.0f) || mx > 3.0e38f) return 0;
+    return max(-100, (int) ((__float_as_uint(mx) >> 23) & 255u) - 127 - 8);
+}
+__device__ __forceinline__ float pg_pow2(int e) { return __uint_as_float((unsigned) (e + 127) << 23); }   // -126 <= e <= 127
+
+__device__ __forceinline__ void pg_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// float `p` of this CTA's shared memory, read from the cluster's CTA `rank`
+__device__ __forceinline__ float pg_dsm(const float * p, unsigned rank) {
+    unsigned a = (unsigned) __cvta_generic_to_shared(p), r;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+    return v;
+}
+
+__host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? 4 : 3; }
+__host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D) * 2 * PD_TK * D * 2; }
+
+// grid = (splits, n_kv_head, n), clusters of `splits` CTAs, 128 threads
+template <class QT, class CT, int D, int MT>
+__global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAttn a) {
+    constexpr bool F32 = sizeof(QT) == 4;
+    constexpr int RPM = F32 ? 8 : 16;              // queries of an M tile
+    constexpr int NS = pd_stages(D), KS = D / 16, CH = D / 8;
+    constexpr int TILE = PD_TK * D * 2;            // bytes of a K or a V tile
+    constexpr float BIAS = PgBias<CT>::v;
+    extern __shared__ __align__(128) unsigned char pd_sm[];
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    const int i = blockIdx.z, h = blockIdx.y, rank = blockIdx.x, nrank = gridDim.x, g = a.group;
+
+    const int len = __ldg(a.len + i), px = pg_prefix_of(a, i);
+    const int plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
+    if (len < 0 || len > (a.max_blocks << a.page_log2) || plen < 0 || plen > (a.prefix_max_blocks << a.page_log2)) {
+        if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
+        return;                                    // the whole cluster: it shares i
+    }
+    const int np = (plen + PD_TK - 1) / PD_TK, total = np + (len + PD_TK - 1) / PD_TK;
+    const int per = (total + nrank - 1) / nrank, t_beg = min(total, rank * per), t_end = min(total, t_beg + per);
+    const int mine = t_end - t_beg > w ? (t_end - t_beg - w + PD_WARPS - 1) / PD_WARPS : 0;   // tiles of this warp
+
+    // page ids of the warp's next 16 tiles, one per lane and 8-key half: tile
+    // x's halves are lanes 2 (x % 16) and 2 (x % 16) + 1; -1 where no key is
+    auto fetch_ids = [&](int x0) {
+        const int x = x0 + (lane >> 1);
+        int id = -1;
+        if (x < mine) {
+            const int t = t_beg + w + x * PD_WARPS;
+            const bool pre = t < np;
+            const int key = (pre ? t : t - np) * PD_TK + (lane & 1) * 8;
+            if (key < (pre ? plen : len)) {
+                id = __ldg((pre ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) i * a.max_blocks) +
+                           (key >> a.page_log2));
+                if ((unsigned) id >= (unsigned) a.n_pages) { atomicOr(&g_paged_err, T3B_DEVERR_PAGE); id = -1; }
+            }
+        }
+        return id;
+    };
+    int ids = fetch_ids(0), ids_next = -1;
+
+    const unsigned ring = (unsigned) __cvta_generic_to_shared(pd_sm) + w * NS * 2 * TILE;
+    // keys that tile x's half holds (0 .. 8)
+    auto half_keys = [&](int x, int half, int id) {
+        const int t = t_beg + w + x * PD_WARPS;
+        const int left = (t < np ? plen - t * PD_TK : len - (t - np) * PD_TK) - half * 8;
+        return id < 0 ? 0 : min(8, left);
+    };
+    auto issue = [&](int x, int my_ids) {          // tile x's K and V into stage x % NS
+        if (x < mine) {
+            const int t = t_beg + w + x * PD_WARPS, key0 = (t < np ? t : t - np) * PD_TK;
+            const unsigned st = ring + (x % NS) * 2 * TILE;
+#pragma unroll
+            for (int c = 0; c < PD_TK * CH / 32; ++c) {
+                const int q = lane + c * 32, row = q / CH, ch = q % CH;
+                const int id = __shfl_sync(0xffffffffu, my_ids, 2 * (x & 15) + (row >> 3));
+                const bool on = (row & 7) < half_keys(x, row >> 3, id);
+                const int key = key0 + row;
+                const long long off = on ? (long long) id * a.page_stride +
+                                               (((long long) h << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D + ch * 8
+                                         : 0;
+                const unsigned d = st + row * (D * 2) + ((ch ^ (row & 7)) << 4);
+                pg_cp16(d, (const CT *) a.k + off, on);
+                pg_cp16(d + TILE, (const CT *) a.v + off, on);   // keys past the end are zeros: 0 * NaN would stay
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int x = 0; x < NS - 1; ++x) issue(x, ids);
+
+    // queries as A fragments
+    unsigned qf[MT][KS][4];
+    float sc[MT][2];                               // what a score of row lane / 4 (+ 8) is multiplied by
+    const float sl2 = a.scale * 1.4426950408889634f;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        if (F32) {
+            const int r = mt * RPM + (lane >> 2);
+            const float * q = (const float *) a.q + (long long) i * a.q_stride + (h * g + min(r, g - 1)) * D;
+            float2 v[KS][2];
+            float mx = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    v[k][b] = *(const float2 *) (q + k * 16 + b * 8 + (lane & 3) * 2);
+                    if (r >= g) v[k][b] = make_float2(0.f, 0.f);
+                    v[k][b].x *= sl2; v[k][b].y *= sl2;
+                    mx = fmaxf(mx, fmaxf(fabsf(v[k][b].x), fabsf(v[k][b].y)));
+                }
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const int e = pg_row_exp(mx);
+            const float f = pg_pow2(-e);
+            sc[mt][0] = sc[mt][1] = pg_pow2(e);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) pg_split2(v[k][b].x * f, v[k][b].y * f, qf[mt][k][2 * b], qf[mt][k][2 * b + 1]);
+        } else {
+            sc[mt][0] = sc[mt][1] = sl2;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int r = mt * RPM + (lane >> 2) + (b & 1) * 8;
+                    qf[mt][k][b] = r < g ? *(const unsigned *) ((const CT *) a.q + (long long) i * a.q_stride + (h * g + r) * D +
+                                                                k * 16 + (b >> 1) * 8 + (lane & 3) * 2)
+                                         : 0u;
+                }
+        }
+    }
+
+    float o[MT][D / 8][4];
+    float m[MT][2], l[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        m[mt][0] = m[mt][1] = -INFINITY; l[mt][0] = l[mt][1] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
+    }
+    const int lr = lane & 7, mi = lane >> 3;       // ldmatrix: row of matrix mi
+    for (int x = 0; x < mine; ++x) {
+        // stage x + NS - 1 is the one that tile x - 1 has left; its ids may be of the next batch
+        const int xn = x + NS - 1;
+        if ((x & 15) == 0) ids_next = fetch_ids(x + 16);
+        issue(xn, (xn >> 4) == (x >> 4) ? ids : ids_next);
+        asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
+        __syncwarp();
+        const int n0 = half_keys(x, 0, __shfl_sync(0xffffffffu, ids, 2 * (x & 15)));
+        const int n1 = half_keys(x, 1, __shfl_sync(0xffffffffu, ids, 2 * (x & 15) + 1));
+        const unsigned st = ring + (x % NS) * 2 * TILE;
+        float s[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            unsigned b[4];
+            const int row = (mi >> 1) * 8 + lr, ch = k * 2 + (mi & 1);
+            pg_ldm4(b, st + row * (D * 2) + ((ch ^ lr) << 4));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                pg_mma<CT>(s[mt][0], qf[mt][k], b[0], b[1]);
+                pg_mma<CT>(s[mt][1], qf[mt][k], b[2], b[3]);
+            }
+        }
+        unsigned p[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float z[2][4];                         // scores in units of log2, masked
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float raw = F32 ? s[mt][nt][e & 1] + s[mt][nt][(e & 1) + 2] : s[mt][nt][e];
+                    z[nt][e] = (lane & 3) * 2 + (e & 1) < (nt ? n1 : n0) ? raw * sc[mt][e >> 1] : -INFINITY;
+                }
+            float top[2];
+            bool grow = false;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                float t = fmaxf(fmaxf(z[0][2 * r], z[0][2 * r + 1]), fmaxf(z[1][2 * r], z[1][2 * r + 1]));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+                t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+                top[r] = fmaxf(m[mt][r], t);
+                grow |= top[r] > m[mt][r] + PD_LAZY;   // also from -inf
+            }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float c = m[mt][r] == -INFINITY ? 0.0f : pg_exp2(m[mt][r] - top[r]);
+                    m[mt][r] = top[r]; l[mt][r] *= c;
+#pragma unroll
+                    for (int d = 0; d < D / 8; ++d) { o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c; }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float base = m[mt][r] == -INFINITY ? 0.0f : m[mt][r] - BIAS;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    z[nt][2 * r] = pg_exp2(z[nt][2 * r] - base);
+                    z[nt][2 * r + 1] = pg_exp2(z[nt][2 * r + 1] - base);
+                    l[mt][r] += z[nt][2 * r] + z[nt][2 * r + 1];
+                }
+            }
+            if (F32) {
+                pg_split2(z[0][0], z[0][1], p[mt][0], p[mt][1]);
+                pg_split2(z[1][0], z[1][1], p[mt][2], p[mt][3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[mt][e] = pg_pack2<CT>(z[e >> 1][2 * (e & 1)], z[e >> 1][2 * (e & 1) + 1]);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < KS; ++d) {
+            unsigned b[4];
+            const int row = (mi & 1) * 8 + lr, ch = d * 2 + (mi >> 1);
+            pg_ldm4t(b, st + TILE + row * (D * 2) + ((ch ^ lr) << 4));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                pg_mma<CT>(o[mt][2 * d], p[mt], b[0], b[1]);
+                pg_mma<CT>(o[mt][2 * d + 1], p[mt], b[2], b[3]);
+            }
+        }
+        __syncwarp();
+        if ((x & 15) == 15) ids = ids_next;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+
+    // join the warps: each leaves (o, m, l) of the group's queries
+    float * so = (float *) pd_sm;                  // [PD_WARPS][g][D]
+    float * sm = so + PD_WARPS * g * D;            // [PD_WARPS][g]
+    float * ss = sm + PD_WARPS * g;                // [PD_WARPS][g]
+    float * co = ss + PD_WARPS * g;                // [g][D], the CTA's
+    float * cm = co + g * D, * cl = cm + g;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < (F32 ? 1 : 2); ++r) {
+            const int q = mt * RPM + (lane >> 2) + r * 8;
+            l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 1);
+            l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 2);
+            if (q < g) {
+#pragma unroll
+                for (int d = 0; d < D / 8; ++d) {
+                    const float2 v = F32 ? make_float2(o[mt][d][0] + o[mt][d][2], o[mt][d][1] + o[mt][d][3])
+                                         : make_float2(o[mt][d][2 * r], o[mt][d][2 * r + 1]);
+                    *(float2 *) (so + (w * g + q) * D + d * 8 + (lane & 3) * 2) = v;
+                }
+                if ((lane & 3) == 0) { sm[w * g + q] = m[mt][r]; ss[w * g + q] = l[mt][r]; }
+            }
+        }
+    __syncthreads();
+    for (int x = tid; x < g * D; x += 32 * PD_WARPS) {
+        const int q = x / D;
+        float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
+#pragma unroll
+        for (int y = 0; y < PD_WARPS; ++y) mx = fmaxf(mx, sm[y * g + q]);
+#pragma unroll
+        for (int y = 0; y < PD_WARPS; ++y) {
+            const float c = sm[y * g + q] == -INFINITY ? 0.0f : pg_exp2(sm[y * g + q] - mx);
+            ov += c * so[y * g * D + x];
+            lv += c * ss[y * g + q];
+        }
+        co[x] = ov;
+        if (x % D == 0) { cm[q] = mx; cl[q] = lv; }
+    }
+    if (nrank > 1) pg_cluster_sync(); else __syncthreads();
+    // join the cluster's CTAs, each an equal share of the outputs
+    QT * out = (QT *) a.out + (long long) i * a.out_stride + h * g * D;
+    for (int x = rank * 32 * PD_WARPS + tid; x < g * D; x += nrank * 32 * PD_WARPS) {
+        const int q = x / D;
+        float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
+        for (int y = 0; y < nrank; ++y) {
+            const float my = pg_dsm(cm + q, y), oy = pg_dsm(co + x, y), ly = pg_dsm(cl + q, y);
+            const float mn = fmaxf(mx, my);
+            const float c = mx == -INFINITY ? 0.0f : pg_exp2(mx - mn), d = my == -INFINITY ? 0.0f : pg_exp2(my - mn);
+            ov = ov * c + oy * d; lv = lv * c + ly * d;
+            mx = mn;
+        }
+        out[x] = pg_from<QT>(lv == 0.0f ? 0.0f : ov / lv);
+    }
+    if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -361,6 +720,46 @@ PgAttn pg_args(const t3b_shared_attn & a, bool prompt) {
     return p;
 }
 
+// CTAs of a (request, kv head): enough that the grid fills the GPU about four
+// times over, while each still has 256 keys
+int pg_splits(const t3b_shared_attn & a) {
+    const int64_t units = (int64_t) a.n * a.cache.n_kv_head;
+    const int64_t keys = ((int64_t) a.max_blocks + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
+    int c = 1;
+    while (c < 8 && units * c < 4 * 148 && keys > (int64_t) 256 * c) c *= 2;
+    return c;
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device.
+template <class K> cudaError_t pg_allow_smem(K * kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <class QT, class CT, int D, int MT>
+cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
+    const cudaError_t e = pg_allow_smem(attn_shared_decode_kernel<QT, CT, D, MT>, pd_smem(D));
+    if (e != cudaSuccess) return e;
+    const unsigned c = (unsigned) pg_splits(a);
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(c, (unsigned) p.n_kv_head, (unsigned) p.n); cfg.blockDim = dim3(32 * PD_WARPS);
+    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
+}
+
+template <class QT, class CT, int D>
+cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, bool prompt, cudaStream_t st) {
+    if (!prompt) {
+        // F32 queries take two of an M tile's 16 rows
+        if (sizeof(QT) == 4 && p.group > 8) return pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st);
+        return pg_launch_decode<QT, CT, D, 1>(a, p, st);
+    }
+    attn_shared_simple_kernel<QT, CT, D><<<dim3(p.rows, p.n_head), 128, 0, st>>>(p);
+    return cudaGetLastError();
+}
+
 int pg_attention(const char * name, const t3b_shared_attn * a, bool prompt, void * cuda_stream) {
     if (!a) { set_err(nullptr, "%s: null argument", name); return T3B_ERR_ARG; }
     if (const char * w = pg_attn_wrong(*a, prompt, true)) { set_err(nullptr, "%s: %s", name, w); return T3B_ERR_ARG; }
@@ -372,20 +771,16 @@ int pg_attention(const char * name, const t3b_shared_attn * a, bool prompt, void
     if (a->rows == 0) return T3B_OK;
     cudaStream_t st = (cudaStream_t) cuda_stream;
     const PgAttn p = pg_args(*a, prompt);
-    const dim3 grid(a->rows, a->n_head);
-    const int D = a->cache.head_dim;
-    if (a->dtype == T3B_F32) {
-        if (D == 64) attn_shared_simple_kernel<float, __half, 64><<<grid, 128, 0, st>>>(p);
-        else attn_shared_simple_kernel<float, __half, 128><<<grid, 128, 0, st>>>(p);
-    } else if (a->dtype == T3B_F16) {
-        if (D == 64) attn_shared_simple_kernel<__half, __half, 64><<<grid, 128, 0, st>>>(p);
-        else attn_shared_simple_kernel<__half, __half, 128><<<grid, 128, 0, st>>>(p);
-    } else {
-        if (D == 64) attn_shared_simple_kernel<__nv_bfloat16, __nv_bfloat16, 64><<<grid, 128, 0, st>>>(p);
-        else attn_shared_simple_kernel<__nv_bfloat16, __nv_bfloat16, 128><<<grid, 128, 0, st>>>(p);
-    }
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) { set_err(nullptr, "%s: %s", name, cudaGetErrorString(e)); return T3B_ERR_CUDA; }
+    const bool wide = a->cache.head_dim == 128;
+    cudaError_t e;
+    if (a->dtype == T3B_F32)
+        e = wide ? pg_launch_attention<float, __half, 128>(*a, p, prompt, st) : pg_launch_attention<float, __half, 64>(*a, p, prompt, st);
+    else if (a->dtype == T3B_F16)
+        e = wide ? pg_launch_attention<__half, __half, 128>(*a, p, prompt, st) : pg_launch_attention<__half, __half, 64>(*a, p, prompt, st);
+    else
+        e = wide ? pg_launch_attention<__nv_bfloat16, __nv_bfloat16, 128>(*a, p, prompt, st)
+                 : pg_launch_attention<__nv_bfloat16, __nv_bfloat16, 64>(*a, p, prompt, st);
+    if (e != cudaSuccess) { set_err(nullptr, "%s: %s", name, cudaGetErrorString(e)); (void) cudaGetLastError(); return T3B_ERR_CUDA; }
     return T3B_OK;
 }
 
