@@ -208,6 +208,7 @@ struct PgAttn {
     const int * len, * table, * row_start, * prefix_start, * prefix_len, * prefix_table;
     int n, rows, n_head, n_kv_head, group, page_log2, n_pages, max_blocks, n_prefix, prefix_max_blocks;
     float scale;
+    float * part;   // prefix parts of a decode batch: [n][n_head][D + 4] floats, (O, max, sum)
 };
 
 // the prefix whose range holds request i, or -1
@@ -221,74 +222,36 @@ __device__ __forceinline__ int pg_prefix_of(const PgAttn & a, int i) {
     return lo - 1;
 }
 
-// The plain form: one CTA per (row, head), its warps striding the keys, each
-// lane holding D / 32 dimensions, every key's dot product added over the
-// warp.
-template <class T, class C, int D>
-__global__ __launch_bounds__(128) void attn_shared_simple_kernel(PgAttn a) {
+// One row and head by one warp, key by key in 32 bits: lane x ends with
+// elements x * D / 32 .. of the output.  The tiled prompt kernel comes here
+// for rows whose output is not finite: a NaN or infinity in the V of a later
+// token that the row does not see meets a probability of zero in its tile.
+template <class QT, class CT, int D>
+__device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, int px, int plen, int own, int kvh, float (&o)[D / 32]) {
     constexpr int E = D / 32;
-    __shared__ float sm_m[4], sm_l[4], sm_o[4][D];
-    const int h = blockIdx.y, r = blockIdx.x, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int i = r, add = 1, at = 0;
-    if (a.row_start) {
-        if (r >= __ldg(a.row_start + a.n)) return;
-        int lo = 0, hi = a.n;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (__ldg(a.row_start + mid) <= r) lo = mid; else hi = mid;
-        }
-        i = lo;
-        add = __ldg(a.row_start + i + 1) - __ldg(a.row_start + i);
-        at = r - __ldg(a.row_start + i);
-    }
-    const int len = __ldg(a.len + i), px = pg_prefix_of(a, i);
-    const int plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
-    const bool one = a.row_start == nullptr;
-    if (len < 0 || len > (a.max_blocks << a.page_log2) || plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
-        (!one && (add <= 0 || add > len || at < 0))) {
-        if (threadIdx.x == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
-        return;
-    }
-    const int own = one ? len : len - add + at + 1, total = plen + own;
-    const int kvh = h / a.group;
-    const T * q = (const T *) a.q + (long long) r * a.q_stride + h * D;
-    float qv[E], o[E];
+    const int lane = threadIdx.x & 31;
+    float qv[E], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; ++e) { qv[e] = pg_to(q[lane * E + e]); o[e] = 0.0f; }
-    float m = -INFINITY, l = 0.0f;
-    for (int j = w; j < total; j += 4) {
+    for (int j = 0; j < plen + own; ++j) {
         const int t = j < plen ? j : j - plen;
-        const int * tab = j < plen ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) i * a.max_blocks;
-        const int id = __ldg(tab + (t >> a.page_log2));
-        if ((unsigned) id >= (unsigned) a.n_pages) { if (lane == 0) atomicOr(&g_paged_err, T3B_DEVERR_PAGE); continue; }
+        const int id = __ldg((j < plen ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) i * a.max_blocks) +
+                             (t >> a.page_log2));
+        if ((unsigned) id >= (unsigned) a.n_pages) continue;
         const long long off = (long long) id * a.page_stride +
                               (((long long) kvh << a.page_log2) + (t & ((1 << a.page_log2) - 1))) * D + lane * E;
-        const C * kp = (const C *) a.k + off, * vp = (const C *) a.v + off;
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(qv[e], pg_to(kp[e]), s);
+        for (int e = 0; e < E; ++e) s = fmaf(qv[e], pg_to(((const CT *) a.k)[off + e]), s);
         s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = expf(s - mn);
+        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = mn == -INFINITY ? 0.0f : expf(s - mn);
         l = l * c + p;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * pg_to(vp[e]);
+        for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * pg_to(((const CT *) a.v)[off + e]);
         m = mn;
     }
-    if (lane == 0) { sm_m[w] = m; sm_l[w] = l; }
 #pragma unroll
-    for (int e = 0; e < E; ++e) sm_o[w][lane * E + e] = o[e];
-    __syncthreads();
-    const float mx = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
-    T * out = (T *) a.out + (long long) r * a.out_stride + h * D;
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float ls = 0.0f, os = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const float c = sm_m[x] == -INFINITY ? 0.0f : expf(sm_m[x] - mx);
-            ls += c * sm_l[x]; os += c * sm_o[x][d];
-        }
-        out[d] = pg_from<T>(ls > 0.0f ? os / ls : 0.0f);
-    }
+    for (int e = 0; e < E; ++e) o[e] = l == 0.0f ? 0.0f : o[e] / l;
 }
 
 // ---- decode: one query token per request -----------------------------------
@@ -649,6 +612,553 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
     if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
 }
 
+// ---- many rows: tcgen05 tiles ------------------------------------------------
+//
+// 256 rows (token x head of the group) against 128-key tiles, for prompt
+// chunks and for the prefix of a decode batch.  Compute-bound: 4 D operations
+// per row and key.  Two 128-row tiles take turns: while the tensor cores work
+// on one, eight warps (a thread per row) run the softmax of the other, so
+// one K / V tile in shared memory serves 256 rows.
+//
+// * Four loader warps bring K and V tiles into a ring by cp.async, 16 bytes at
+//   a time, in the 128-byte swizzle (panels of 64 dimensions x 128 keys):
+//   page boundaries, ragged ends (zero-filled) and absent pages are a matter
+//   of each row's source address.
+// * One thread issues the MMAs.  S = Q K^T (both K-major in shared memory) goes
+//   to tensor memory; the softmax threads read it, write P over it, and P V
+//   takes P from tensor memory and V as the MN-major operand.  MMAs of one
+//   thread execute in issue order, so Q K^T of the next tile may follow P V
+//   into the same columns.
+// * O stays in tensor memory and is rescaled only when a row's maximum has
+//   grown by 2^8 since the last time (as in the decode kernel).
+// * F32 queries are two f16 parts, and so are their probabilities: two MMAs
+//   into one accumulator.
+// * The keys of a tile of rows may be split over a cluster (few rows, many
+//   keys); its CTAs join their (O, max, sum) over distributed shared memory.
+//
+// Every wait has a limit (TF_SPIN polls); one that runs out ends the loops of
+// its role, the others' waits run out in turn, and the call is reported.
+#define PT_ROWS 256
+#define PT_BN 128
+#define PT_THREADS 416          // warps 0-7 softmax, 8 MMA, 9-12 loaders
+#define PT_PANEL (128 * 128)    // bytes of 128 rows x 64 elements
+
+__host__ __device__ constexpr int pt_slots(int D, bool f32) { return D == 128 && f32 ? 3 : 4; }
+__host__ __device__ constexpr int pt_q_bytes(int D, bool f32) { return 2 * (f32 ? 2 : 1) * (D / 64) * PT_PANEL; }
+__host__ __device__ constexpr int pt_ring_bytes(int D, bool f32) { return pt_slots(D, f32) * (D / 64) * PT_PANEL; }
+__host__ __device__ constexpr int pt_smem(int D, bool f32) {
+    // the epilogue puts [256][D + 4] floats and two per row over Q and the ring, which are larger
+    return 1024 + pt_q_bytes(D, f32) + pt_ring_bytes(D, f32);
+}
+
+#define PG_R32(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define PG_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+// 32 columns of this warp's 32 lanes (a row per thread); pg_tm_wait_ld before use
+__device__ __forceinline__ void pg_tm_ld32(unsigned (&r)[32], unsigned addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : PG_R32(r, 0), PG_R32(r, 8), PG_R32(r, 16), PG_R32(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pg_tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pg_tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pg_tm_st32(const unsigned (&r)[32], unsigned addr) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+                 ::"r"(addr), PG_W8(r, 0), PG_W8(r, 8), PG_W8(r, 16), PG_W8(r, 24) : "memory");
+}
+__device__ __forceinline__ void pg_tm_st16(const unsigned (&r)[16], unsigned addr) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 ::"r"(addr), PG_W8(r, 0), PG_W8(r, 8) : "memory");
+}
+__device__ __forceinline__ void pg_commit(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool pg_test(unsigned bar, unsigned parity) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done;
+}
+__device__ __forceinline__ void pg_arrive(unsigned bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void pg_mma_ss(unsigned d, unsigned long long da, unsigned long long db, unsigned idesc, unsigned acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned long long db, unsigned idesc, unsigned acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+                 ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(acc) : "memory");
+}
+
+// A tile of rows: rows lo .. lo + count - 1 of the `total` rows (token x
+// head) of request i (prompt) or of prefix px's requests (its part of a
+// decode batch), whose first token is row `row0` of q.
+struct PgTile { int i, px, row0, total, lo; };
+
+// The z-th 256-row tile over all requests (prompt) or prefixes, found by one
+// warp; false past the last one.  Requests whose rows are out of range are
+// passed over.
+template <bool PARTIAL>
+__device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
+    const int lane = threadIdx.x & 31, n = PARTIAL ? a.n_prefix : a.n;
+    const int * start = PARTIAL ? a.prefix_start : a.row_start;
+    const int most = PARTIAL ? a.n : a.rows;
+    int before = 0;
+    for (int b = 0; b < n; b += 32) {
+        const int x = b + lane;
+        int beg = 0, cnt = 0;
+        if (x < n) {
+            beg = __ldg(start + x); cnt = __ldg(start + x + 1) - beg;
+            if (beg < 0 || cnt < 0 || cnt > most - beg) {
+                if (z == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
+                cnt = 0;
+            }
+        }
+        const int mine = (int) (((long long) cnt * a.group + PT_ROWS - 1) / PT_ROWS);
+        int inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const int sum = __shfl_sync(0xffffffffu, inc, 31);
+        if (z < before + sum) {
+            const unsigned hit = __ballot_sync(0xffffffffu, z < before + inc);
+            const int l = __ffs(hit) - 1;
+            t.i = t.px = b + l;
+            t.row0 = __shfl_sync(0xffffffffu, beg, l);
+            t.total = __shfl_sync(0xffffffffu, cnt, l) * a.group;
+            t.lo = (z - before - __shfl_sync(0xffffffffu, inc - mine, l)) * PT_ROWS;
+            if (!PARTIAL) t.px = pg_prefix_of(a, t.i);
+            return true;
+        }
+        before += sum;
+    }
+    return false;
+}
+
+static_assert(pt_smem(64, false) >= 1024 + PT_ROWS * (64 + 6) * 4 && pt_smem(128, false) >= 1024 + PT_ROWS * (128 + 6) * 4, "epilogue");
+
+// grid = (tiles x splits, n_kv_head), clusters of `splits` CTAs.  PARTIAL: the
+// prefix keys for all of a decode batch's rows, (O, max, sum) to the
+// workspace; otherwise a prompt's rows, prefix and own keys, to `out`.
+template <class QT, class CT, int D, bool PARTIAL>
+__global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn a) {
+    constexpr bool F32 = sizeof(QT) == 4;
+    constexpr int NP = D / 64, R = pt_slots(D, F32), PARTS = F32 ? 2 : 1;
+    constexpr int SLOT = NP * PT_PANEL, QTILE = PARTS * SLOT;     // bytes
+    constexpr float BIAS = PgBias<CT>::v;
+    constexpr unsigned FMT = std::is_same<CT, __half>::value ? 0u : (1u << 7) | (1u << 10);
+    constexpr unsigned ID_QK = (1u << 4) | FMT | ((unsigned) (PT_BN >> 3) << 17) | (8u << 24);
+    constexpr unsigned ID_PV = (1u << 4) | FMT | (1u << 16) | ((unsigned) (D >> 3) << 17) | (8u << 24);   // B is MN-major
+    extern __shared__ __align__(16) unsigned char pt_raw[];
+    unsigned char * sm = pt_raw + ((1024u - ((unsigned) __cvta_generic_to_shared(pt_raw) & 1023u)) & 1023u);
+    const unsigned smq = (unsigned) __cvta_generic_to_shared(sm), smr = smq + 2 * QTILE;
+    __shared__ __align__(8) unsigned long long bars[2 * R + 6];
+    __shared__ unsigned s_mask[4][4], s_tmem;
+    __shared__ PgTile s_tile;
+    __shared__ int s_have, s_bad;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    float * so = (float *) sm, * s_m = so + PT_ROWS * (D + 4), * s_l = s_m + PT_ROWS;   // epilogue: over Q and the ring
+    int rank, nrank;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
+    const int h = blockIdx.y, g = a.group;
+    const unsigned bar0 = (unsigned) __cvta_generic_to_shared(bars);
+    auto full = [&](int s) { return bar0 + 8 * s; };
+    auto empty = [&](int s) { return bar0 + 8 * (R + s); };
+    auto s_full = [&](int t) { return bar0 + 8 * (2 * R + t); };
+    auto p_full = [&](int t) { return bar0 + 8 * (2 * R + 2 + t); };
+    const unsigned q_full = bar0 + 8 * (2 * R + 4), o_full = bar0 + 8 * (2 * R + 5);
+
+    if (PARTIAL) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 0) {
+        PgTile t{};
+        const bool have = pg_find_tile<PARTIAL>(a, blockIdx.x / nrank, t);
+        if (lane == 0) { s_have = have; s_tile = t; s_bad = 0; }
+    }
+    if (tid == 32) {
+        for (int s = 0; s < R; ++s) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" ::"r"(full(s)) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty(s)) : "memory");
+        }
+        for (int t = 0; t < 2; ++t) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_full(t)) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(p_full(t)) : "memory");
+        }
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(q_full) : "memory");
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(o_full) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (!s_have) return;                           // the whole cluster: it shares the tile
+    const PgTile t = s_tile;
+    const int px = t.px, plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
+    const int cnt = min(PT_ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
+    const int add = t.total / g, len = PARTIAL ? 0 : __ldg(a.len + t.i);
+    if (plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
+        (!PARTIAL && (len < 0 || len > (a.max_blocks << a.page_log2) || add > len))) {
+        if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
+        return;                                    // (PARTIAL: the decode kernel leaves these requests alone too)
+    }
+    // own keys that the tile's last row sees, key tiles of this CTA
+    const int seen = PARTIAL ? 0 : len - add + (t.lo + cnt - 1) / g + 1;
+    const int np = (plen + PT_BN - 1) / PT_BN, all = np + (seen + PT_BN - 1) / PT_BN;
+    const int per = (all + nrank - 1) / nrank, kt0 = min(all, rank * per), nk = min(all, kt0 + per) - kt0;
+
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 256 + D x
+
+    if (warp < 8) {
+        // ---------------- softmax: thread = row ----------------
+        const int x = warp >> 2, r = tid & 255, row = t.lo + r;   // tile, row of the CTA, row of the request
+        const bool live = r < cnt;
+        const int tok = row / g, head = h * g + row % g;
+        const QT * q = (const QT *) a.q + (long long) (t.row0 + (live ? tok : 0)) * a.q_stride + (live ? head : 0) * D;
+        const float sl2 = fabsf(a.scale) * 1.4426950408889634f;
+        float sc = sl2;
+        if (x < nt) {
+            const unsigned qd = smq + x * QTILE, rr = r & 127;
+            if (F32) {
+                const float c = a.scale * 1.4426950408889634f;
+                float mx = 0.0f;
+                if (live)
+#pragma unroll 8
+                    for (int e = 0; e < D / 4; ++e) {
+                        const float4 v = __ldg((const float4 *) q + e);
+                        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x * c)), fmaxf(fabsf(v.y * c), fabsf(v.z * c))), fabsf(v.w * c));
+                    }
+                const int ex = pg_row_exp(mx);
+                const float f = pg_pow2(-ex);
+                sc = pg_pow2(ex);
+#pragma unroll 4
+                for (int e = 0; e < D / 8; ++e) {
+                    float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+                    if (live) { u = __ldg((const float4 *) q + 2 * e); v = __ldg((const float4 *) q + 2 * e + 1); }
+                    uint4 hi, lo;
+                    pg_split2(u.x * c * f, u.y * c * f, hi.x, lo.x); pg_split2(u.z * c * f, u.w * c * f, hi.y, lo.y);
+                    pg_split2(v.x * c * f, v.y * c * f, hi.z, lo.z); pg_split2(v.z * c * f, v.w * c * f, hi.w, lo.w);
+                    const unsigned off = (e >> 3) * PT_PANEL + rr * 128 + (((e & 7) ^ (rr & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qd + off), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qd + SLOT + off), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+                }
+            } else {
+                const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale is folded into q
+#pragma unroll 8
+                for (int e = 0; e < D / 8; ++e) {
+                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                    if (live) v = __ldg((const uint4 *) q + e);
+                    const unsigned off = (e >> 3) * PT_PANEL + rr * 128 + (((e & 7) ^ (rr & 7)) << 4);
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                 ::"r"(qd + off), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        pg_arrive(q_full);
+
+        float m = -INFINITY, l = 0.0f;
+        bool ok = true;
+        const unsigned lanes = tm + ((unsigned) ((warp & 3) * 32) << 16), ts = lanes + 128 * x, to = lanes + 256 + D * x;
+        const int lim_own = PARTIAL ? 0 : len - add + tok + 1;      // own keys that this row sees
+        if (x < nt) {
+            for (int j = 0; j < nk; ++j) {
+                ok = tf_wait(s_full(x), (unsigned) j & 1u);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const int kt = kt0 + j;
+                const int left = kt < np ? PT_BN : lim_own - (kt - np) * PT_BN;   // keys of the tile before the causal limit
+                unsigned msk[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int v = left - 32 * c;
+                    msk[c] = s_mask[kt & 3][c] & (v >= 32 ? 0xffffffffu : v <= 0 ? 0u : (1u << v) - 1u);
+                }
+                const bool plain = __all_sync(0xffffffffu, (msk[0] & msk[1] & msk[2] & msk[3]) == 0xffffffffu);
+                float top = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    unsigned u[32], v[32];
+                    pg_tm_ld32(u, ts + 32 * c);
+                    pg_tm_ld32(v, ts + 32 * c + 32);
+                    pg_tm_wait_ld();
+                    if (!plain) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            if (!(msk[c] >> e & 1u)) u[e] = 0xff800000u;
+                            if (!(msk[c + 1] >> e & 1u)) v[e] = 0xff800000u;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaxf(__uint_as_float(u[e]), __uint_as_float(v[e])));
+                }
+                top = fmaxf(m, top * sc);          // sc > 0; -inf stays
+                if (__any_sync(0xffffffffu, top > m + PD_LAZY)) {
+                    const float f = m == -INFINITY ? 0.0f : pg_exp2(m - top);
+                    m = top; l *= f;
+                    if (j > 0)
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            unsigned u[32];
+                            pg_tm_ld32(u, to + c);
+                            pg_tm_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
+                            pg_tm_st32(u, to + c);
+                        }
+                }
+                const float base = m == -INFINITY ? 0.0f : m - BIAS;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    unsigned u[32];
+                    pg_tm_ld32(u, ts + 32 * c);
+                    pg_tm_wait_ld();
+                    float pv[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) pv[e] = pg_exp2(fmaf(__uint_as_float(u[e]), sc, -base));
+                    if (!plain)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) if (!(msk[c] >> e & 1u)) pv[e] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) l += (pv[e] + pv[e + 1]) + (pv[e + 2] + pv[e + 3]);
+                    unsigned hi[16], lo[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (F32) pg_split2(pv[2 * e], pv[2 * e + 1], hi[e], lo[e]);
+                        else hi[e] = pg_pack2<CT>(pv[2 * e], pv[2 * e + 1]);
+                    }
+                    // P lies over the columns of S that were read: 16 per 32 keys, F32's lo parts right behind
+                    pg_tm_st16(hi, ts + (F32 ? 32 : 16) * c);
+                    if (F32) pg_tm_st16(lo, ts + 32 * c + 16);
+                }
+                pg_tm_wait_st();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                pg_arrive(p_full(x));
+            }
+            if (nk > 0 && ok) ok = tf_wait(o_full, 0u);
+            ok = __all_sync(0xffffffffu, ok);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (!ok) s_bad = 1;
+        // (O, max, sum) of the row into shared memory, over Q and the ring:
+        // o_full means that every MMA of the CTA has read them
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (x < nt) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                unsigned u[32];
+                if (nk > 0) {
+                    pg_tm_ld32(u, to + c);
+                    pg_tm_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) u[e] = 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *(uint4 *) (so + r * (D + 4) + c + e) = make_uint4(u[e], u[e + 1], u[e + 2], u[e + 3]);
+            }
+            s_m[r] = m; s_l[r] = l;
+        }
+    } else if (warp == 8) {
+        // ---------------- MMA issue ----------------
+        if (lane == 0) {
+            auto desc_k = [](unsigned addr) { return tf_desc(addr); };                       // K-major, see the F16 GEMM
+            auto desc_mn = [](unsigned addr) {                                              // MN-major: 64-element panels LBO apart
+                return (tf_desc(addr) & ~(0x3fffull << 16)) | ((unsigned long long) (PT_PANEL >> 4) << 16);
+            };
+            auto qk = [&](int x, int n) {           // S of tile x = Q K^T, K in item n's slot
+                const unsigned ka = smr + (n % R) * SLOT, qa = smq + x * QTILE;
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const unsigned off = (k >> 2) * PT_PANEL + (k & 3) * 32;
+                        pg_mma_ss(tm + 128 * x, desc_k(qa + part * SLOT + off), desc_k(ka + off), ID_QK, part || k ? 1u : 0u);
+                    }
+                pg_commit(s_full(x));
+            };
+            auto pv = [&](int x, int n, bool first) {
+                const unsigned va = smr + (n % R) * SLOT;
+#pragma unroll
+                for (int k = 0; k < PT_BN / 16; ++k)
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        pg_mma_ts(tm + 256 + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k),
+                                  desc_mn(va + k * 2048), ID_PV, first && k == 0 && part == 0 ? 0u : 1u);
+            };
+            bool ok = tf_wait(q_full, 0u);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (nk > 0 && ok) {
+                ok = tf_wait(full(0), 0u);
+                if (ok) {
+                    for (int x = 0; x < nt; ++x) qk(x, 0);
+                    pg_commit(empty(0));
+                }
+            }
+            for (int j = 0; j < nk && ok; ++j) {
+                const int nv = 2 * j + 1, nn = 2 * j + 2;             // items: V of this tile, K of the next
+                ok = tf_wait(full(nv % R), (unsigned) (nv / R) & 1u);
+                if (ok && j + 1 < nk) ok = tf_wait(full(nn % R), (unsigned) (nn / R) & 1u);
+                for (int x = 0; x < nt && ok; ++x) {
+                    ok = tf_wait(p_full(x), (unsigned) j & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    pv(x, nv, j == 0);
+                    if (x == nt - 1) pg_commit(empty(nv % R));
+                    if (j + 1 < nk) {
+                        qk(x, nn);
+                        if (x == nt - 1) pg_commit(empty(nn % R));
+                    }
+                }
+            }
+            pg_commit(o_full);
+            if (!tf_wait(o_full, 0u) || !ok) s_bad = 1;               // nothing is in flight when the CTA goes on
+        }
+        __syncwarp();
+    } else {
+        // ---------------- loaders: 32 keys of each tile per warp ----------------
+        const int lw = warp - 9;
+        const int items = 2 * nk;
+        auto tile_keys = [&](int kt, int & key0, int & have) {        // first key of tile kt in its segment, keys from it on
+            const bool pre = kt < np;
+            key0 = (pre ? kt : kt - np) * PT_BN;
+            have = (pre ? plen : seen) - key0;
+            return pre;
+        };
+        auto fetch = [&](int kt) {                                    // lane x < 4: the page of keys 8 x .. of this warp's 32
+            int id = -1, key0, have;
+            if (lane < 4 && kt < kt0 + nk) {
+                const bool pre = tile_keys(kt, key0, have);
+                const int k = lw * 32 + lane * 8;
+                if (k < have) {
+                    id = __ldg((pre ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) t.i * a.max_blocks) +
+                               ((key0 + k) >> a.page_log2));
+                    if ((unsigned) id >= (unsigned) a.n_pages) { atomicOr(&g_paged_err, T3B_DEVERR_PAGE); id = -1; }
+                }
+            }
+            return id;
+        };
+        int done = 0;                                                 // items signalled
+        auto signal_to = [&](int upto) {                              // their copies have been waited for
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            for (; done < upto; ++done) if (lane == 0) pg_arrive(full(done % R));
+        };
+        bool ok = true;
+        int ids = fetch(kt0), ids_next = -1;
+        for (int n = 0; n < items && ok; ++n) {
+            const int kt = kt0 + (n >> 1), v = n & 1, s = n % R;
+            if (!v) ids_next = fetch(kt + 1);
+            if (n >= R) {
+                const unsigned ph = (unsigned) (n / R - 1) & 1u;
+                if (!__all_sync(0xffffffffu, pg_test(empty(s), ph))) {
+                    // what is still in flight is waited for first: the MMAs may need it to free the slot
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    signal_to(n);
+                    ok = tf_wait(empty(s), ph);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                }
+            }
+            int key0, have;
+            tile_keys(kt, key0, have);
+            const CT * src = (const CT *) (v ? a.v : a.k);
+            const unsigned slot = smr + s * SLOT;
+            if (!v) {                                                 // which of the 32 keys are there
+                const int gh = min(8, max(0, have - lw * 32 - (lane & 3) * 8));
+                unsigned b = lane < 4 && ids >= 0 ? ((1u << gh) - 1u) << (8 * (lane & 3)) : 0u;
+                b |= __shfl_xor_sync(0xffffffffu, b, 1);
+                b |= __shfl_xor_sync(0xffffffffu, b, 2);
+                if (lane == 0) s_mask[kt & 3][lw] = b;
+            }
+#pragma unroll
+            for (int it = 0; it < 8; ++it) {
+                const int rr = it * 4 + (lane >> 3), krow = lw * 32 + rr, c = lane & 7;
+                const int id = __shfl_sync(0xffffffffu, ids, it >> 1);
+                const bool on = id >= 0 && krow < have;
+                const int key = key0 + krow;
+                const long long off = on ? (long long) id * a.page_stride +
+                                               (((long long) h << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D + c * 8
+                                         : 0;
+                const unsigned d = slot + krow * 128 + ((c ^ (krow & 7)) << 4);
+#pragma unroll
+                for (int p = 0; p < NP; ++p) pg_cp16(d + p * PT_PANEL, src + off + (on ? p * 64 : 0), on);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (v) ids = ids_next;
+            if (n > done) {                                           // all but the newest item have arrived
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                signal_to(n);
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (ok) signal_to(items); else s_bad = 1;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 8) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+    }
+    if (s_bad && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_TIMEOUT);
+    if (nrank > 1) pg_cluster_sync();
+
+    // join the cluster's parts and write: a warp per row
+    constexpr int E = D / 32;
+    for (int r = rank + nrank * warp; r < cnt; r += nrank * (PT_THREADS / 32)) {
+        float mx = -INFINITY, lv = 0.0f, ov[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) ov[e] = 0.0f;
+        for (int y = 0; y < nrank; ++y) {
+            float my, ly, oy[E];
+            if (nrank > 1) {
+                my = pg_dsm(s_m + r, y); ly = pg_dsm(s_l + r, y);
+#pragma unroll
+                for (int e = 0; e < E; ++e) oy[e] = pg_dsm(so + r * (D + 4) + lane * E + e, y);
+            } else {
+                my = s_m[r]; ly = s_l[r];
+#pragma unroll
+                for (int e = 0; e < E; ++e) oy[e] = so[r * (D + 4) + lane * E + e];
+            }
+            const float mn = fmaxf(mx, my);
+            const float c = mx == -INFINITY ? 0.0f : pg_exp2(mx - mn), d = my == -INFINITY ? 0.0f : pg_exp2(my - mn);
+            lv = lv * c + ly * d;
+#pragma unroll
+            for (int e = 0; e < E; ++e) ov[e] = ov[e] * c + oy[e] * d;
+            mx = mn;
+        }
+        const int row = t.lo + r, tok = row / g, head = h * g + row % g;
+        if (PARTIAL) {
+            float * rec = a.part + ((long long) (t.row0 + tok) * a.n_head + head) * (D + 4);
+#pragma unroll
+            for (int e = 0; e < E; ++e) rec[lane * E + e] = ov[e];
+            if (lane == 0) { rec[D] = mx; rec[D + 1] = lv; }
+        } else {
+            bool fine = true;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                ov[e] = lv == 0.0f ? 0.0f : ov[e] / lv;
+                fine = fine && fabsf(ov[e]) < INFINITY;
+            }
+            if (!__all_sync(0xffffffffu, fine))
+                pg_row_slow<QT, CT, D>(a, (const QT *) a.q + (long long) (t.row0 + tok) * a.q_stride + head * D, t.i, px, plen,
+                                       len - add + tok + 1, h, ov);
+            QT * out = (QT *) a.out + (long long) (t.row0 + tok) * a.out_stride + head * D;
+#pragma unroll
+            for (int e = 0; e < E; ++e) out[lane * E + e] = pg_from<QT>(ov[e]);
+        }
+    }
+    if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -749,6 +1259,26 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
 }
 
+template <class QT, class CT, int D, bool PARTIAL>
+cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
+    constexpr bool F32 = sizeof(QT) == 4;
+    const cudaError_t e = pg_allow_smem(attn_shared_tile_kernel<QT, CT, D, PARTIAL>, pt_smem(D, F32));
+    if (e != cudaSuccess) return e;
+    // each request (prefix) may end in a part-filled tile
+    const int64_t parts = PARTIAL ? p.n_prefix : p.n, rows = PARTIAL ? p.n : p.rows;
+    const int64_t tiles = std::min((rows * p.group + PT_ROWS - 1) / PT_ROWS + parts, rows * p.group);
+    const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
+    int c = 1;
+    while (c < 8 && tiles * p.n_kv_head * 2 * c <= 148 && keys > (int64_t) 2 * PT_BN * c) c *= 2;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned) c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned) (tiles * c), (unsigned) p.n_kv_head); cfg.blockDim = dim3(PT_THREADS);
+    cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL>, p);
+}
+
 template <class QT, class CT, int D>
 cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, bool prompt, cudaStream_t st) {
     if (!prompt) {
@@ -756,8 +1286,7 @@ cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, boo
         if (sizeof(QT) == 4 && p.group > 8) return pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st);
         return pg_launch_decode<QT, CT, D, 1>(a, p, st);
     }
-    attn_shared_simple_kernel<QT, CT, D><<<dim3(p.rows, p.n_head), 128, 0, st>>>(p);
-    return cudaGetLastError();
+    return pg_launch_tiles<QT, CT, D, false>(a, p, st);
 }
 
 int pg_attention(const char * name, const t3b_shared_attn * a, bool prompt, void * cuda_stream) {

@@ -336,6 +336,32 @@ def test_scale_argument(pkg, prompt, scale):
     _close(b, scale=scale)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_values_of_later_tokens_stay_there(pkg, kind, value):
+    """A NaN or infinity in the K or V of a token reaches the rows that see it, and no row before it."""
+    b = Batch(kind, [100, 30], 6, 2, 64, 16, [70], [0, 2], adds=[60, 30], seed=31)
+    ref, tol = b.reference()
+    key = 85                                                      # own key 85 of request 0: rows from 45 on see it
+    slot = int(b.table[0, key // 16]), key % 16
+    for pool, dims in ((b.v, slice(3, 5)), (b.k, slice(9, 10))):
+        view = pool.view(b.n_pages, b.kv, 16, 64)
+        old = view[slot[0], 1, slot[1]].clone()
+        view[slot[0], 1, slot[1], dims] = value                   # kv head 1: query heads 3, 4 and 5
+        b.out_all.fill_(-7)
+        _attend(pkg, b)
+        view[slot[0], 1, slot[1]] = old
+        got = b.out_all[:90].cpu().double()
+        clean = torch.ones_like(ref, dtype=torch.bool)
+        clean[45:60, 3 * 64:] = False
+        assert ((got - ref).abs() <= tol)[clean].all()
+        if pool is b.v:
+            hit = got[45:60].view(15, 6, 64)[:, 3:, dims]
+            assert (~torch.isfinite(hit)).all()
+            if value != value:
+                assert torch.isnan(hit).all()
+
+
 @pytest.mark.parametrize("prompt", [False, True])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_output_in_place_of_q(pkg, prompt, kind):
