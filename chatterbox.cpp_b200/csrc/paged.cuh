@@ -357,10 +357,11 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
     const int len = __ldg(a.len + i), px = pg_prefix_of(a, i);
     const int plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
     if (len < 0 || len > (a.max_blocks << a.page_log2) || plen < 0 || plen > (a.prefix_max_blocks << a.page_log2)) {
+        if (a.part) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
         return;                                    // the whole cluster: it shares i
     }
-    const int np = (plen + PD_TK - 1) / PD_TK, total = np + (len + PD_TK - 1) / PD_TK;
+    const int np = a.part ? 0 : (plen + PD_TK - 1) / PD_TK, total = np + (len + PD_TK - 1) / PD_TK;
     const int per = (total + nrank - 1) / nrank, t_beg = min(total, rank * per), t_end = min(total, t_beg + per);
     const int mine = t_end - t_beg > w ? (t_end - t_beg - w + PD_WARPS - 1) / PD_WARPS : 0;   // tiles of this warp
 
@@ -594,12 +595,17 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         co[x] = ov;
         if (x % D == 0) { cm[q] = mx; cl[q] = lv; }
     }
+    if (a.part) asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix parts are there
     if (nrank > 1) pg_cluster_sync(); else __syncthreads();
-    // join the cluster's CTAs, each an equal share of the outputs
+    // join the prefix's part and the cluster's CTAs, each an equal share of the outputs
     QT * out = (QT *) a.out + (long long) i * a.out_stride + h * g * D;
     for (int x = rank * 32 * PD_WARPS + tid; x < g * D; x += nrank * 32 * PD_WARPS) {
         const int q = x / D;
         float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
+        if (a.part && px >= 0) {
+            const float * rec = a.part + ((long long) i * a.n_head + h * g + q) * (D + 4);
+            mx = __ldcg(rec + D); lv = __ldcg(rec + D + 1); ov = __ldcg(rec + x % D);
+        }
         for (int y = 0; y < nrank; ++y) {
             const float my = pg_dsm(cm + q, y), oy = pg_dsm(co + x, y), ly = pg_dsm(cl + q, y);
             const float mn = fmaxf(mx, my);
@@ -1215,7 +1221,19 @@ const char * pg_attn_wrong(const t3b_shared_attn & a, bool prompt, bool pointers
     return nullptr;
 }
 
-size_t pg_workspace(const t3b_shared_attn & a, bool prompt) { (void) a; (void) prompt; return 0; }
+// Whether a decode call computes its prefixes' attention once for the batch
+// (the tile kernel, then joined by the decode kernel) or lets every request
+// read its prefix through L2.
+bool pg_shares(const t3b_shared_attn & a) {
+    if (a.n_prefix == 0) return false;
+    const char * e = getenv("PGS");
+    if (e) return atoi(e);
+    return true;
+}
+
+size_t pg_workspace(const t3b_shared_attn & a, bool prompt) {
+    return !prompt && pg_shares(a) ? (size_t) a.n * a.n_head * (a.cache.head_dim + 4) * sizeof(float) : 0;
+}
 
 PgAttn pg_args(const t3b_shared_attn & a, bool prompt) {
     PgAttn p{};
@@ -1226,6 +1244,7 @@ PgAttn pg_args(const t3b_shared_attn & a, bool prompt) {
     p.n = a.n; p.rows = a.rows; p.n_head = a.n_head; p.n_kv_head = a.cache.n_kv_head; p.group = a.n_head / a.cache.n_kv_head;
     pg_log2(a.cache.page_size, 3, 8, &p.page_log2);
     p.n_pages = a.cache.n_pages; p.max_blocks = a.max_blocks; p.n_prefix = a.n_prefix; p.prefix_max_blocks = a.prefix_max_blocks;
+    p.part = pg_workspace(a, prompt) ? (float *) a.workspace : nullptr;
     p.scale = a.scale != 0.0f ? a.scale : 1.0f / sqrtf((float) a.cache.head_dim);
     return p;
 }
@@ -1234,7 +1253,7 @@ PgAttn pg_args(const t3b_shared_attn & a, bool prompt) {
 // times over, while each still has 256 keys
 int pg_splits(const t3b_shared_attn & a) {
     const int64_t units = (int64_t) a.n * a.cache.n_kv_head;
-    const int64_t keys = ((int64_t) a.max_blocks + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
+    const int64_t keys = ((int64_t) a.max_blocks + (a.n_prefix > 0 && !pg_shares(a) ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     int c = 1;
     while (c < 8 && units * c < 4 * 148 && keys > (int64_t) 256 * c) c *= 2;
     return c;
@@ -1251,11 +1270,13 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     if (e != cudaSuccess) return e;
     const unsigned c = (unsigned) pg_splits(a);
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // runs beside the tile kernel that comes before it
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(c, (unsigned) p.n_kv_head, (unsigned) p.n); cfg.blockDim = dim3(32 * PD_WARPS);
-    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = p.part ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
 }
 
@@ -1282,6 +1303,10 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
 template <class QT, class CT, int D>
 cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, bool prompt, cudaStream_t st) {
     if (!prompt) {
+        if (p.part) {
+            const cudaError_t e = pg_launch_tiles<QT, CT, D, true>(a, p, st);
+            if (e != cudaSuccess) return e;
+        }
         // F32 queries take two of an M tile's 16 rows
         if (sizeof(QT) == 4 && p.group > 8) return pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st);
         return pg_launch_decode<QT, CT, D, 1>(a, p, st);
