@@ -646,7 +646,8 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 // its role, the others' waits run out in turn, and the call is reported.
 #define PT_ROWS 256
 #define PT_BN 128
-#define PT_THREADS 416          // warps 0-7 softmax, 8 MMA, 9-12 loaders
+#define PT_THREADS 384          // warps 0-7 softmax, 8 MMA, 9-11 loaders: three warps a scheduler, 168 registers
+#define PT_LOADERS 3
 #define PT_PANEL (128 * 128)    // bytes of 128 rows x 64 elements
 
 __host__ __device__ constexpr int pt_slots(int D, bool f32) { return D == 128 && f32 ? 3 : 4; }
@@ -657,24 +658,26 @@ __host__ __device__ constexpr int pt_smem(int D, bool f32) {
     return 1024 + pt_q_bytes(D, f32) + pt_ring_bytes(D, f32);
 }
 
-#define PG_R32(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define PG_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define PG_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
 // 32 columns of this warp's 32 lanes (a row per thread); pg_tm_wait_ld before use
 __device__ __forceinline__ void pg_tm_ld32(unsigned (&r)[32], unsigned addr) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                  "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-                 : PG_R32(r, 0), PG_R32(r, 8), PG_R32(r, 16), PG_R32(r, 24) : "r"(addr) : "memory");
+                 : PG_R8(r, 0), PG_R8(r, 8), PG_R8(r, 16), PG_R8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pg_tm_ld16(unsigned (&r)[16], unsigned addr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : PG_R8(r, 0), PG_R8(r, 8) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void pg_tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pg_tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pg_tm_st32(const unsigned (&r)[32], unsigned addr) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-                 ::"r"(addr), PG_W8(r, 0), PG_W8(r, 8), PG_W8(r, 16), PG_W8(r, 24) : "memory");
-}
 __device__ __forceinline__ void pg_tm_st16(const unsigned (&r)[16], unsigned addr) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  ::"r"(addr), PG_W8(r, 0), PG_W8(r, 8) : "memory");
+}
+__device__ __forceinline__ void pg_sts(unsigned addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void pg_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -761,8 +764,9 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
     extern __shared__ __align__(16) unsigned char pt_raw[];
     unsigned char * sm = pt_raw + ((1024u - ((unsigned) __cvta_generic_to_shared(pt_raw) & 1023u)) & 1023u);
     const unsigned smq = (unsigned) __cvta_generic_to_shared(sm), smr = smq + 2 * QTILE;
-    __shared__ __align__(8) unsigned long long bars[2 * R + 6];
-    __shared__ unsigned s_mask[4][4], s_tmem;
+    __shared__ __align__(8) unsigned long long bars[2 * R + 8];
+    __shared__ __align__(16) unsigned char s_mask[4][16];      // keys present in 8-key groups, of the last four tiles
+    __shared__ unsigned s_tmem;
     __shared__ PgTile s_tile;
     __shared__ int s_have, s_bad;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -776,7 +780,8 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
     auto empty = [&](int s) { return bar0 + 8 * (R + s); };
     auto s_full = [&](int t) { return bar0 + 8 * (2 * R + t); };
     auto p_full = [&](int t) { return bar0 + 8 * (2 * R + 2 + t); };
-    const unsigned q_full = bar0 + 8 * (2 * R + 4), o_full = bar0 + 8 * (2 * R + 5);
+    auto p_half = [&](int t) { return bar0 + 8 * (2 * R + 4 + t); };
+    const unsigned q_full = bar0 + 8 * (2 * R + 6), o_full = bar0 + 8 * (2 * R + 7);
 
     if (PARTIAL) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
@@ -786,12 +791,13 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
     }
     if (tid == 32) {
         for (int s = 0; s < R; ++s) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], 4;" ::"r"(full(s)) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(s)), "n"(PT_LOADERS) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(empty(s)) : "memory");
         }
         for (int t = 0; t < 2; ++t) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s_full(t)) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(p_full(t)) : "memory");
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(p_half(t)) : "memory");
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(q_full) : "memory");
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(o_full) : "memory");
@@ -826,45 +832,67 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
     if (warp < 8) {
         // ---------------- softmax: thread = row ----------------
         const int x = warp >> 2, r = tid & 255, row = t.lo + r;   // tile, row of the CTA, row of the request
-        const bool live = r < cnt;
-        const int tok = row / g, head = h * g + row % g;
-        const QT * q = (const QT *) a.q + (long long) (t.row0 + (live ? tok : 0)) * a.q_stride + (live ? head : 0) * D;
+        const int tok = row / g;
         const float sl2 = fabsf(a.scale) * 1.4426950408889634f;
-        float sc = sl2;
+        float sc = sl2;                            // what the row's scores are multiplied by
         if (x < nt) {
-            const unsigned qd = smq + x * QTILE, rr = r & 127;
-            if (F32) {
-                const float c = a.scale * 1.4426950408889634f;
-                float mx = 0.0f;
-                if (live)
-#pragma unroll 8
-                    for (int e = 0; e < D / 4; ++e) {
-                        const float4 v = __ldg((const float4 *) q + e);
-                        mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v.x * c)), fmaxf(fabsf(v.y * c), fabsf(v.z * c))), fabsf(v.w * c));
-                    }
-                const int ex = pg_row_exp(mx);
-                const float f = pg_pow2(-ex);
-                sc = pg_pow2(ex);
-#pragma unroll 4
-                for (int e = 0; e < D / 8; ++e) {
-                    float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-                    if (live) { u = __ldg((const float4 *) q + 2 * e); v = __ldg((const float4 *) q + 2 * e + 1); }
-                    uint4 hi, lo;
-                    pg_split2(u.x * c * f, u.y * c * f, hi.x, lo.x); pg_split2(u.z * c * f, u.w * c * f, hi.y, lo.y);
-                    pg_split2(v.x * c * f, v.y * c * f, hi.z, lo.z); pg_split2(v.z * c * f, v.w * c * f, hi.w, lo.w);
-                    const unsigned off = (e >> 3) * PT_PANEL + rr * 128 + (((e & 7) ^ (rr & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qd + off), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w) : "memory");
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qd + SLOT + off), "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w) : "memory");
+            // The warp stages its 32 rows, eight lanes to 64 elements: lane c
+            // of a row's eight brings 16 bytes of each panel.
+            const unsigned qd = smq + x * QTILE;
+            const int c = lane & 7;
+            const float cs = a.scale * 1.4426950408889634f;
+            const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale is folded into q
+#pragma unroll
+            for (int b = 0; b < 8; b += 4) {       // four rows of each lane group in flight
+                float4 v[4][NP][PARTS];            // F32: eight floats, else eight 16-bit values in [0]
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rw = (r & ~31) + (b + k) * 4 + (lane >> 3), rq = t.lo + rw;
+                    const QT * q = (const QT *) a.q + (long long) (t.row0 + rq / g) * a.q_stride + (h * g + rq % g) * D + c * 8;
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+#pragma unroll
+                        for (int y = 0; y < PARTS; ++y)
+                            v[k][p][y] = rw < cnt ? __ldg((const float4 *) (q + p * 64) + y) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
-            } else {
-                const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale is folded into q
-#pragma unroll 8
-                for (int e = 0; e < D / 8; ++e) {
-                    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                    if (live) v = __ldg((const uint4 *) q + e);
-                    const unsigned off = (e >> 3) * PT_PANEL + rr * 128 + (((e & 7) ^ (rr & 7)) << 4);
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                 ::"r"(qd + off), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int rr = ((r & ~31) + (b + k) * 4 + (lane >> 3)) & 127;
+                    const unsigned off = rr * 128 + ((c ^ (rr & 7)) << 4);
+                    if (F32) {
+                        float mx = 0.0f;
+#pragma unroll
+                        for (int p = 0; p < NP; ++p)
+#pragma unroll
+                            for (int y = 0; y < PARTS; ++y) {
+                                float4 & w = v[k][p][y];
+                                w.x *= cs; w.y *= cs; w.z *= cs; w.w *= cs;
+                                mx = fmaxf(fmaxf(fmaxf(mx, fabsf(w.x)), fmaxf(fabsf(w.y), fabsf(w.z))), fabsf(w.w));
+                            }
+#pragma unroll
+                        for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const int ex = pg_row_exp(mx);
+                        const float f = pg_pow2(-ex), back = pg_pow2(ex);
+                        // the thread of row 4 (b + k) + y is lane 4 (b + k) + y; the row's scale is in lanes 8 y ..
+                        const float mine = __shfl_sync(0xffffffffu, back, (lane & 3) * 8);
+                        if ((lane >> 2) == b + k) sc = mine;
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) {
+                            const float4 u = v[k][p][0], w = v[k][p][PARTS - 1];
+                            uint4 hi, lo;
+                            pg_split2(u.x * f, u.y * f, hi.x, lo.x); pg_split2(u.z * f, u.w * f, hi.y, lo.y);
+                            pg_split2(w.x * f, w.y * f, hi.z, lo.z); pg_split2(w.z * f, w.w * f, hi.w, lo.w);
+                            pg_sts(qd + p * PT_PANEL + off, hi);
+                            pg_sts(qd + SLOT + p * PT_PANEL + off, lo);
+                        }
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) {
+                            const float4 u = v[k][p][0];
+                            pg_sts(qd + p * PT_PANEL + off, make_uint4(__float_as_uint(u.x) ^ flip, __float_as_uint(u.y) ^ flip,
+                                                                       __float_as_uint(u.z) ^ flip, __float_as_uint(u.w) ^ flip));
+                        }
+                    }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -882,68 +910,64 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int kt = kt0 + j;
                 const int left = kt < np ? PT_BN : lim_own - (kt - np) * PT_BN;   // keys of the tile before the causal limit
-                unsigned msk[4];
+                unsigned u[4][32];                 // the row's scores
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int v = left - 32 * c;
-                    msk[c] = s_mask[kt & 3][c] & (v >= 32 ? 0xffffffffu : v <= 0 ? 0u : (1u << v) - 1u);
-                }
-                const bool plain = __all_sync(0xffffffffu, (msk[0] & msk[1] & msk[2] & msk[3]) == 0xffffffffu);
-                float top = -INFINITY;
+                for (int c = 0; c < 4; ++c) pg_tm_ld32(u[c], ts + 32 * c);
+                const uint4 here = *(const uint4 *) s_mask[kt & 3];
+                pg_tm_wait_ld();
+                const bool whole = (here.x & here.y & here.z & here.w) == 0xffffffffu && left >= PT_BN;
+                if (!__all_sync(0xffffffffu, whole)) {
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    unsigned u[32], v[32];
-                    pg_tm_ld32(u, ts + 32 * c);
-                    pg_tm_ld32(v, ts + 32 * c + 32);
-                    pg_tm_wait_ld();
-                    if (!plain) {
+                    for (int c = 0; c < 4; ++c) {
+                        const int v = left - 32 * c;
+                        const unsigned word = c == 0 ? here.x : c == 1 ? here.y : c == 2 ? here.z : here.w;
+                        const unsigned msk = word & (v >= 32 ? 0xffffffffu : v <= 0 ? 0u : (1u << v) - 1u);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            if (!(msk[c] >> e & 1u)) u[e] = 0xff800000u;
-                            if (!(msk[c + 1] >> e & 1u)) v[e] = 0xff800000u;
-                        }
+                        for (int e = 0; e < 32; ++e) if (!(msk >> e & 1u)) u[c][e] = 0xff800000u;
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) top = fmaxf(top, fmaxf(__uint_as_float(u[e]), __uint_as_float(v[e])));
                 }
-                top = fmaxf(m, top * sc);          // sc > 0; -inf stays
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tops[c] = fmaxf(tops[c], __uint_as_float(u[c][e]));
+                const float top = fmaxf(m, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * sc);   // sc > 0; -inf stays
                 if (__any_sync(0xffffffffu, top > m + PD_LAZY)) {
                     const float f = m == -INFINITY ? 0.0f : pg_exp2(m - top);
                     m = top; l *= f;
                     if (j > 0)
-#pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            unsigned u[32];
-                            pg_tm_ld32(u, to + c);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            unsigned w[16];
+                            pg_tm_ld16(w, to + c);
                             pg_tm_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * f);
-                            pg_tm_st32(u, to + c);
+                            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+                            pg_tm_st16(w, to + c);
                         }
                 }
                 const float base = m == -INFINITY ? 0.0f : m - BIAS;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    unsigned u[32];
-                    pg_tm_ld32(u, ts + 32 * c);
-                    pg_tm_wait_ld();
-                    float pv[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) pv[e] = pg_exp2(fmaf(__uint_as_float(u[e]), sc, -base));
-                    if (!plain)
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) if (!(msk[c] >> e & 1u)) pv[e] = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) l += (pv[e] + pv[e + 1]) + (pv[e + 2] + pv[e + 3]);
+                    float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                     unsigned hi[16], lo[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        if (F32) pg_split2(pv[2 * e], pv[2 * e + 1], hi[e], lo[e]);
-                        else hi[e] = pg_pack2<CT>(pv[2 * e], pv[2 * e + 1]);
+                        const float p0 = pg_exp2(fmaf(__uint_as_float(u[c][2 * e]), sc, -base));
+                        const float p1 = pg_exp2(fmaf(__uint_as_float(u[c][2 * e + 1]), sc, -base));
+                        ls[2 * (e & 1)] += p0; ls[2 * (e & 1) + 1] += p1;
+                        if (F32) pg_split2(p0, p1, hi[e], lo[e]);
+                        else hi[e] = pg_pack2<CT>(p0, p1);
                     }
-                    // P lies over the columns of S that were read: 16 per 32 keys, F32's lo parts right behind
+                    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                    // P lies over the columns of S: 16 per 32 keys, F32's lo parts right behind
                     pg_tm_st16(hi, ts + (F32 ? 32 : 16) * c);
                     if (F32) pg_tm_st16(lo, ts + 32 * c + 16);
+                    if (c == 1) {                  // the first 64 keys' P V may begin
+                        pg_tm_wait_st();
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        pg_arrive(p_half(x));
+                    }
                 }
                 pg_tm_wait_st();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -992,10 +1016,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
                     }
                 pg_commit(s_full(x));
             };
-            auto pv = [&](int x, int n, bool first) {
+            auto pv = [&](int x, int n, bool first, int half) {   // P V over half of the tile's keys
                 const unsigned va = smr + (n % R) * SLOT;
 #pragma unroll
-                for (int k = 0; k < PT_BN / 16; ++k)
+                for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
 #pragma unroll
                     for (int part = 0; part < PARTS; ++part)
                         pg_mma_ts(tm + 256 + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k),
@@ -1015,10 +1039,14 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
                 ok = tf_wait(full(nv % R), (unsigned) (nv / R) & 1u);
                 if (ok && j + 1 < nk) ok = tf_wait(full(nn % R), (unsigned) (nn / R) & 1u);
                 for (int x = 0; x < nt && ok; ++x) {
+                    ok = tf_wait(p_half(x), (unsigned) j & 1u);
+                    if (!ok) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    pv(x, nv, j == 0, 0);
                     ok = tf_wait(p_full(x), (unsigned) j & 1u);
                     if (!ok) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    pv(x, nv, j == 0);
+                    pv(x, nv, false, 1);
                     if (x == nt - 1) pg_commit(empty(nv % R));
                     if (j + 1 < nk) {
                         qk(x, nn);
@@ -1031,7 +1059,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
         }
         __syncwarp();
     } else {
-        // ---------------- loaders: 32 keys of each tile per warp ----------------
+        // ---------------- loaders: every third group of 8 keys per warp ----------------
         const int lw = warp - 9;
         const int items = 2 * nk;
         auto tile_keys = [&](int kt, int & key0, int & have) {        // first key of tile kt in its segment, keys from it on
@@ -1040,11 +1068,11 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
             have = (pre ? plen : seen) - key0;
             return pre;
         };
-        auto fetch = [&](int kt) {                                    // lane x < 4: the page of keys 8 x .. of this warp's 32
+        auto fetch = [&](int kt) {                                    // lane x < 16: the page of keys 8 x ..
             int id = -1, key0, have;
-            if (lane < 4 && kt < kt0 + nk) {
+            if (lane < 16 && kt < kt0 + nk) {
                 const bool pre = tile_keys(kt, key0, have);
-                const int k = lw * 32 + lane * 8;
+                const int k = lane * 8;
                 if (k < have) {
                     id = __ldg((pre ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) t.i * a.max_blocks) +
                                ((key0 + k) >> a.page_log2));
@@ -1078,25 +1106,23 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
             tile_keys(kt, key0, have);
             const CT * src = (const CT *) (v ? a.v : a.k);
             const unsigned slot = smr + s * SLOT;
-            if (!v) {                                                 // which of the 32 keys are there
-                const int gh = min(8, max(0, have - lw * 32 - (lane & 3) * 8));
-                unsigned b = lane < 4 && ids >= 0 ? ((1u << gh) - 1u) << (8 * (lane & 3)) : 0u;
-                b |= __shfl_xor_sync(0xffffffffu, b, 1);
-                b |= __shfl_xor_sync(0xffffffffu, b, 2);
-                if (lane == 0) s_mask[kt & 3][lw] = b;
-            }
+            if (!v && lane < 16 && lane % PT_LOADERS == lw)           // which keys of its groups are there
+                s_mask[kt & 3][lane] = ids >= 0 ? (unsigned char) ((1u << min(8, max(0, have - lane * 8))) - 1u) : (unsigned char) 0;
 #pragma unroll
-            for (int it = 0; it < 8; ++it) {
-                const int rr = it * 4 + (lane >> 3), krow = lw * 32 + rr, c = lane & 7;
-                const int id = __shfl_sync(0xffffffffu, ids, it >> 1);
-                const bool on = id >= 0 && krow < have;
-                const int key = key0 + krow;
-                const long long off = on ? (long long) id * a.page_stride +
-                                               (((long long) h << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D + c * 8
-                                         : 0;
-                const unsigned d = slot + krow * 128 + ((c ^ (krow & 7)) << 4);
+            for (int gi = 0; gi < (16 + PT_LOADERS - 1) / PT_LOADERS; ++gi) {
+                const int grp = gi * PT_LOADERS + lw;
+                if (grp >= 16) break;
+                const int id = __shfl_sync(0xffffffffu, ids, grp);
+                const long long page = id >= 0 ? (long long) id * a.page_stride + ((long long) h << a.page_log2) * D : 0;
 #pragma unroll
-                for (int p = 0; p < NP; ++p) pg_cp16(d + p * PT_PANEL, src + off + (on ? p * 64 : 0), on);
+                for (int y = 0; y < 2; ++y) {
+                    const int krow = grp * 8 + y * 4 + (lane >> 3), c = lane & 7;
+                    const bool on = id >= 0 && krow < have;
+                    const CT * from = src + (on ? page + ((key0 + krow) & ((1 << a.page_log2) - 1)) * D + c * 8 : 0);
+                    const unsigned d = slot + krow * 128 + ((c ^ (krow & 7)) << 4);
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) pg_cp16(d + p * PT_PANEL, from + (on ? p * 64 : 0), on);
+                }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
             if (v) ids = ids_next;
