@@ -626,10 +626,12 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 // on one, eight warps (a thread per row) run the softmax of the other, so
 // one K / V tile in shared memory serves 256 rows.
 //
-// * Four loader warps bring K and V tiles into a ring by cp.async, 16 bytes at
-//   a time, in the 128-byte swizzle (panels of 64 dimensions x 128 keys):
-//   page boundaries, ragged ends (zero-filled) and absent pages are a matter
-//   of each row's source address.
+// * Three loader warps bring K and V tiles into a ring in the 128-byte swizzle
+//   (panels of 64 dimensions x 128 keys): a tile whose 128 keys are all there
+//   by TMA, a box per page and panel; a ragged one by cp.async, 16 bytes at a
+//   time, where the end (zero-filled: what lies behind it may be NaN) and absent
+//   pages are a matter of each row's source address.  cp.async alone bounded
+//   the loop: 1200 cycles to issue a 32 KB item, against a handful for TMA.
 // * One thread issues the MMAs.  S = Q K^T (both K-major in shared memory) goes
 //   to tensor memory; the softmax threads read it, write P over it, and P V
 //   takes P from tensor memory and V as the MN-major operand.  MMAs of one
@@ -700,25 +702,32 @@ __device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned long 
                  ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(acc) : "memory");
 }
 
-// A tile of rows: rows lo .. lo + count - 1 of the `total` rows (token x
-// head) of request i (prompt) or of prefix px's requests (its part of a
-// decode batch), whose first token is row `row0` of q.
-struct PgTile { int i, px, row0, total, lo; };
+// A tile of rows: rows lo .. of the `total` rows (token x head) of request i
+// (prompt) or of prefix px's requests (its part of a decode batch), whose
+// first token is row `row0` of q; lengths of the prefix (px < 0: none) and of
+// the own keys (PARTIAL: none).
+struct PgTile { int i, px, row0, total, lo, plen, len; };
 
 // The z-th 256-row tile over all requests (prompt) or prefixes, found by one
 // warp; false past the last one.  Requests whose rows are out of range are
-// passed over.
+// passed over.  What the tile needs of its request is loaded beside the
+// starts, and up to 32 prefixes beside those: one trip to memory.
 template <bool PARTIAL>
 __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     const int lane = threadIdx.x & 31, n = PARTIAL ? a.n_prefix : a.n;
     const int * start = PARTIAL ? a.prefix_start : a.row_start;
+    const int * lens = PARTIAL ? a.prefix_len : a.len;
     const int most = PARTIAL ? a.n : a.rows;
+    int pbeg = 0, pend = 0, pl = 0;
+    if (!PARTIAL && lane < a.n_prefix && a.n_prefix <= 32) {
+        pbeg = __ldg(a.prefix_start + lane); pend = __ldg(a.prefix_start + lane + 1); pl = __ldg(a.prefix_len + lane);
+    }
     int before = 0;
     for (int b = 0; b < n; b += 32) {
         const int x = b + lane;
-        int beg = 0, cnt = 0;
+        int beg = 0, cnt = 0, ln = 0;
         if (x < n) {
-            beg = __ldg(start + x); cnt = __ldg(start + x + 1) - beg;
+            beg = __ldg(start + x); cnt = __ldg(start + x + 1) - beg; ln = __ldg(lens + x);
             if (beg < 0 || cnt < 0 || cnt > most - beg) {
                 if (z == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
                 cnt = 0;
@@ -733,13 +742,23 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
         }
         const int sum = __shfl_sync(0xffffffffu, inc, 31);
         if (z < before + sum) {
-            const unsigned hit = __ballot_sync(0xffffffffu, z < before + inc);
-            const int l = __ffs(hit) - 1;
+            const int l = __ffs(__ballot_sync(0xffffffffu, z < before + inc)) - 1;
             t.i = t.px = b + l;
             t.row0 = __shfl_sync(0xffffffffu, beg, l);
             t.total = __shfl_sync(0xffffffffu, cnt, l) * a.group;
             t.lo = (z - before - __shfl_sync(0xffffffffu, inc - mine, l)) * PT_ROWS;
-            if (!PARTIAL) t.px = pg_prefix_of(a, t.i);
+            t.len = t.plen = __shfl_sync(0xffffffffu, ln, l);
+            if (PARTIAL) {
+                t.len = 0;
+            } else if (a.n_prefix <= 32) {
+                const unsigned in = __ballot_sync(0xffffffffu, pbeg <= t.i && t.i < pend);
+                t.px = __ffs(in) - 1;
+                t.plen = __shfl_sync(0xffffffffu, pl, max(0, t.px));
+                if (!in) t.plen = 0;
+            } else {
+                t.px = pg_prefix_of(a, t.i);
+                t.plen = t.px >= 0 ? __ldg(a.prefix_len + t.px) : 0;
+            }
             return true;
         }
         before += sum;
@@ -753,7 +772,8 @@ static_assert(pt_smem(64, false) >= 1024 + PT_ROWS * (64 + 6) * 4 && pt_smem(128
 // prefix keys for all of a decode batch's rows, (O, max, sum) to the
 // workspace; otherwise a prompt's rows, prefix and own keys, to `out`.
 template <class QT, class CT, int D, bool PARTIAL>
-__global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn a) {
+__global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const __grid_constant__ CUtensorMap mk,
+                                                                         const __grid_constant__ CUtensorMap mv, PgAttn a) {
     constexpr bool F32 = sizeof(QT) == 4;
     constexpr int NP = D / 64, R = pt_slots(D, F32), PARTS = F32 ? 2 : 1;
     constexpr int SLOT = NP * PT_PANEL, QTILE = PARTS * SLOT;     // bytes
@@ -803,22 +823,6 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(o_full) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
-    if (!s_have) return;                           // the whole cluster: it shares the tile
-    const PgTile t = s_tile;
-    const int px = t.px, plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
-    const int cnt = min(PT_ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
-    const int add = t.total / g, len = PARTIAL ? 0 : __ldg(a.len + t.i);
-    if (plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
-        (!PARTIAL && (len < 0 || len > (a.max_blocks << a.page_log2) || add > len))) {
-        if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
-        return;                                    // (PARTIAL: the decode kernel leaves these requests alone too)
-    }
-    // own keys that the tile's last row sees, key tiles of this CTA
-    const int seen = PARTIAL ? 0 : len - add + (t.lo + cnt - 1) / g + 1;
-    const int np = (plen + PT_BN - 1) / PT_BN, all = np + (seen + PT_BN - 1) / PT_BN;
-    const int per = (all + nrank - 1) / nrank, kt0 = min(all, rank * per), nk = min(all, kt0 + per) - kt0;
-
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
                      ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)) : "memory");
@@ -828,6 +832,20 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 256 + D x
+    const PgTile t = s_tile;
+    const int px = t.px, plen = t.plen, len = t.len, add = t.total / g;
+    const bool wrong = plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
+                       (!PARTIAL && (len < 0 || len > (a.max_blocks << a.page_log2) || add > len));
+    if (!s_have || wrong) {                        // the whole cluster: it shares the tile
+        if (s_have && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);   // PARTIAL: the decode kernel leaves these requests alone too
+        if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+        return;
+    }
+    const int cnt = min(PT_ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
+    // own keys that the tile's last row sees, key tiles of this CTA
+    const int seen = PARTIAL ? 0 : len - add + (t.lo + cnt - 1) / g + 1;
+    const int np = (plen + PT_BN - 1) / PT_BN, all = np + (seen + PT_BN - 1) / PT_BN;
+    const int per = (all + nrank - 1) / nrank, kt0 = min(all, rank * per), nk = min(all, kt0 + per) - kt0;
 
     if (warp < 8) {
         // ---------------- softmax: thread = row ----------------
@@ -1106,6 +1124,28 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
             tile_keys(kt, key0, have);
             const CT * src = (const CT *) (v ? a.v : a.k);
             const unsigned slot = smr + s * SLOT;
+            if (have >= PT_BN && (__ballot_sync(0xffffffffu, ids < 0) & 0xffffu) == 0u) {
+                // a whole tile: boxes of a page's keys (at most 128) by TMA, one per lane of the first warp
+                if (done < n) { asm volatile("cp.async.wait_group 0;" ::: "memory"); signal_to(n); }
+                if (!v && lane < 16 && lane % PT_LOADERS == lw) s_mask[kt & 3][lane] = 0xffu;
+                __syncwarp();
+                if (lw == 0) {
+                    const int br = min(1 << a.page_log2, PT_BN), k = lane / NP * br, p = lane % NP;
+                    const int id = __shfl_sync(0xffffffffu, ids, (k >> 3) & 15);
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full(s)), "r"((unsigned) SLOT) : "memory");
+                    __syncwarp();
+                    if (k < PT_BN)
+                        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                                     ::"r"(slot + p * PT_PANEL + k * 128), "l"(v ? &mv : &mk), "r"(p * 64),
+                                       "r"((key0 + k) & ((1 << a.page_log2) - 1)), "r"(h), "r"(id), "r"(full(s)) : "memory");
+                } else if (lane == 0) {
+                    pg_arrive(full(s));
+                }
+                done = n + 1;
+                if (v) ids = ids_next;
+                continue;
+            }
             if (!v && lane < 16 && lane % PT_LOADERS == lw)           // which keys of its groups are there
                 s_mask[kt & 3][lane] = ids >= 0 ? (unsigned char) ((1u << min(8, max(0, have - lane * 8))) - 1u) : (unsigned char) 0;
 #pragma unroll
@@ -1132,7 +1172,11 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(PgAttn 
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (ok) signal_to(items); else s_bad = 1;
+        if (ok) signal_to(items);
+        else {
+            s_bad = 1;                                                // no copy is in flight when the CTA goes on
+            for (int n = max(0, done - R); n < done; ++n) tf_wait(full(n % R), (unsigned) (n / R) & 1u);
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -1211,7 +1255,7 @@ const char * pg_cache_wrong(const t3b_paged_kv & c, bool pointers) {
     if (c.n_pages <= 0 || c.n_kv_head <= 0 || (int64_t) c.n_pages * c.page_size > 0x7fffffffll || c.n_kv_head > 1024)
         return "n_pages or n_kv_head is out of range";
     const int64_t dense = (int64_t) c.n_kv_head * c.page_size * c.head_dim;
-    if (c.page_stride && (c.page_stride < dense || c.page_stride % 8 || c.page_stride > (int64_t) 1 << 40))
+    if (c.page_stride && (c.page_stride < dense || c.page_stride % 8 || c.page_stride >= (int64_t) 1 << 39))
         return "page_stride is below a page's elements or not a multiple of 8";
     if (pointers && (!c.k || !c.v)) return "null cache";
     if (pointers && (!pg_aligned(c.k) || !pg_aligned(c.v))) return "K and V caches must be 16-byte aligned";
@@ -1306,6 +1350,21 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
 }
 
+// The pages of K or V as a 4-D tensor [n_pages][n_kv_head][page][D], boxes of
+// 64 elements x up to 128 keys in the 128-byte swizzle.  Both 16-bit types
+// move as they are.
+bool pg_map(CUtensorMap * map, const void * base, const t3b_paged_kv & c) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc = tf_encode();
+    const cuuint64_t row = (cuuint64_t) c.head_dim * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.page_size, (cuuint64_t) c.n_kv_head, (cuuint64_t) c.n_pages};
+    const cuuint64_t strides[3] = {row, row * c.page_size, (cuuint64_t) pg_page_stride(c) * 2};
+    const cuuint32_t box[4] = {64u, (cuuint32_t) std::min(c.page_size, PT_BN), 1u, 1u};
+    const cuuint32_t es[4] = {1u, 1u, 1u, 1u};
+    return enc && enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void *>(base), dims, strides, box, es,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class QT, class CT, int D, bool PARTIAL>
 cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
     constexpr bool F32 = sizeof(QT) == 4;
@@ -1323,7 +1382,9 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     at[0].val.clusterDim.x = (unsigned) c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned) (tiles * c), (unsigned) p.n_kv_head); cfg.blockDim = dim3(PT_THREADS);
     cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL>, p);
+    CUtensorMap mk, mv;
+    if (!pg_map(&mk, a.cache.k, a.cache) || !pg_map(&mv, a.cache.v, a.cache)) return cudaErrorInvalidValue;
+    return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL>, mk, mv, p);
 }
 
 template <class QT, class CT, int D>
