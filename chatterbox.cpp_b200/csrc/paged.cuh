@@ -681,8 +681,16 @@ __device__ __forceinline__ void pg_tm_st16(const unsigned (&r)[16], unsigned add
 __device__ __forceinline__ void pg_sts(unsigned addr, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void pg_commit(unsigned bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// The MMA warp runs as a whole, so that descriptors and loop state stay in
+// uniform registers, and `el` names the lane that issues.
+__device__ __forceinline__ unsigned pg_elect() {
+    unsigned el;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(el));
+    return el;
+}
+__device__ __forceinline__ void pg_commit(unsigned bar, unsigned el) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(el) : "memory");
 }
 __device__ __forceinline__ bool pg_test(unsigned bar, unsigned parity) {
     unsigned done;
@@ -693,13 +701,22 @@ __device__ __forceinline__ bool pg_test(unsigned bar, unsigned parity) {
 __device__ __forceinline__ void pg_arrive(unsigned bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void pg_mma_ss(unsigned d, unsigned long long da, unsigned long long db, unsigned idesc, unsigned acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(acc) : "memory");
+// Shared-memory descriptors: low word = address / 16 | leading offset / 16 <<
+// 16, high word constant (8-row groups 1024 bytes apart, version 1, 128-byte
+// swizzle; see tf_desc).  K-major operands have no leading offset; the
+// MN-major V steps from panel to panel by it.
+#define PT_DESC_HI ((1024u >> 4) | (1u << 14) | (2u << 29))
+__device__ __forceinline__ void pg_mma_ss(unsigned d, unsigned a, unsigned b, unsigned idesc, unsigned acc, unsigned el) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(el), "r"(PT_DESC_HI) : "memory");
 }
-__device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned long long db, unsigned idesc, unsigned acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-                 ::"r"(d), "r"(a), "l"(db), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned b, unsigned idesc, unsigned acc, unsigned el) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "mov.b64 y, {%2, %6};\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(el), "r"(PT_DESC_HI) : "memory");
 }
 
 // A tile of rows: rows lo .. of the `total` rows (token x head) of request i
@@ -1018,63 +1035,64 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         }
     } else if (warp == 8) {
         // ---------------- MMA issue ----------------
-        if (lane == 0) {
-            auto desc_k = [](unsigned addr) { return tf_desc(addr); };                       // K-major, see the F16 GEMM
-            auto desc_mn = [](unsigned addr) {                                              // MN-major: 64-element panels LBO apart
-                return (tf_desc(addr) & ~(0x3fffull << 16)) | ((unsigned long long) (PT_PANEL >> 4) << 16);
-            };
-            auto qk = [&](int x, int n) {           // S of tile x = Q K^T, K in item n's slot
-                const unsigned ka = smr + (n % R) * SLOT, qa = smq + x * QTILE;
+        const unsigned el = pg_elect();
+        // 14 bits of address: in a cluster, shared addresses carry the CTA's rank above them
+        const unsigned qw = (smq >> 4) & 0x3fffu, rw = (smr >> 4) & 0x3fffu;
+        const unsigned q0 = qw | (1u << 16), k0 = rw | (1u << 16), v0 = rw | ((unsigned) (PT_PANEL >> 4) << 16);
+        auto qk = [&](int x, int slot) {            // S of tile x = Q K^T
+            const unsigned qa = q0 + x * (QTILE >> 4), ka = k0 + slot * (SLOT >> 4);
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const unsigned off = (k >> 2) * (PT_PANEL >> 4) + (k & 3) * 2;
+                    pg_mma_ss(tm + 128 * x, qa + part * (SLOT >> 4) + off, ka + off, ID_QK, part || k ? 1u : 0u, el);
+                }
+            pg_commit(s_full(x), el);
+        };
+        auto pv = [&](int x, int slot, unsigned acc, int half) {   // O of tile x += P V over half of the tile's keys
+            const unsigned va = v0 + slot * (SLOT >> 4);
+#pragma unroll
+            for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const unsigned off = (k >> 2) * PT_PANEL + (k & 3) * 32;
-                        pg_mma_ss(tm + 128 * x, desc_k(qa + part * SLOT + off), desc_k(ka + off), ID_QK, part || k ? 1u : 0u);
-                    }
-                pg_commit(s_full(x));
-            };
-            auto pv = [&](int x, int n, bool first, int half) {   // P V over half of the tile's keys
-                const unsigned va = smr + (n % R) * SLOT;
-#pragma unroll
-                for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
-#pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
-                        pg_mma_ts(tm + 256 + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k),
-                                  desc_mn(va + k * 2048), ID_PV, first && k == 0 && part == 0 ? 0u : 1u);
-            };
-            bool ok = tf_wait(q_full, 0u);
+                    pg_mma_ts(tm + 256 + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k), va + k * 128,
+                              ID_PV, half == 0 && k == 0 && part == 0 ? acc : 1u, el);
+        };
+        bool ok = tf_wait(q_full, 0u);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (nk > 0 && ok) {
+            ok = tf_wait(full(0), 0u);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (nk > 0 && ok) {
-                ok = tf_wait(full(0), 0u);
-                if (ok) {
-                    for (int x = 0; x < nt; ++x) qk(x, 0);
-                    pg_commit(empty(0));
-                }
+            if (ok) {
+                for (int x = 0; x < nt; ++x) qk(x, 0);
+                pg_commit(empty(0), el);
             }
-            for (int j = 0; j < nk && ok; ++j) {
-                const int nv = 2 * j + 1, nn = 2 * j + 2;             // items: V of this tile, K of the next
-                ok = tf_wait(full(nv % R), (unsigned) (nv / R) & 1u);
-                if (ok && j + 1 < nk) ok = tf_wait(full(nn % R), (unsigned) (nn / R) & 1u);
-                for (int x = 0; x < nt && ok; ++x) {
-                    ok = tf_wait(p_half(x), (unsigned) j & 1u);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    pv(x, nv, j == 0, 0);
-                    ok = tf_wait(p_full(x), (unsigned) j & 1u);
-                    if (!ok) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    pv(x, nv, false, 1);
-                    if (x == nt - 1) pg_commit(empty(nv % R));
-                    if (j + 1 < nk) {
-                        qk(x, nn);
-                        if (x == nt - 1) pg_commit(empty(nn % R));
-                    }
-                }
-            }
-            pg_commit(o_full);
-            if (!tf_wait(o_full, 0u) || !ok) s_bad = 1;               // nothing is in flight when the CTA goes on
         }
+        int sv = 1, pv_ph = 0;                      // slot of this tile's V and its phase; K of the next follows
+        for (int j = 0; j < nk && ok; ++j) {
+            const int sk = sv + 1 == R ? 0 : sv + 1, pk_ph = sv + 1 == R ? pv_ph ^ 1 : pv_ph;
+            ok = tf_wait(full(sv), (unsigned) pv_ph);
+            if (ok && j + 1 < nk) ok = tf_wait(full(sk), (unsigned) pk_ph);
+            for (int x = 0; x < nt && ok; ++x) {
+                ok = tf_wait(p_half(x), (unsigned) j & 1u);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                pv(x, sv, j > 0, 0);
+                ok = tf_wait(p_full(x), (unsigned) j & 1u);
+                if (!ok) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                pv(x, sv, 1u, 1);
+                if (x == nt - 1) pg_commit(empty(sv), el);
+                if (j + 1 < nk) {
+                    qk(x, sk);
+                    if (x == nt - 1) pg_commit(empty(sk), el);
+                }
+            }
+            sv = sk + 1 == R ? 0 : sk + 1; pv_ph = sk + 1 == R ? pk_ph ^ 1 : pk_ph;
+        }
+        pg_commit(o_full, el);
+        if (!tf_wait(o_full, 0u) || !ok) s_bad = 1;                   // nothing is in flight when the CTA goes on
         __syncwarp();
     } else {
         // ---------------- loaders: every third group of 8 keys per warp ----------------
