@@ -785,7 +785,8 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
 
 static_assert(pt_smem(64, false) >= 1024 + PT_ROWS * (64 + 6) * 4 && pt_smem(128, false) >= 1024 + PT_ROWS * (128 + 6) * 4, "epilogue");
 
-// grid = (tiles x splits, n_kv_head), clusters of `splits` CTAs.  PARTIAL: the
+// grid = tiles x kv heads x splits, clusters of `splits` CTAs, the last tiles
+// (of a prompt, those with the most keys) first.  PARTIAL: the
 // prefix keys for all of a decode batch's rows, (O, max, sum) to the
 // workspace; otherwise a prompt's rows, prefix and own keys, to `out`.
 template <class QT, class CT, int D, bool PARTIAL>
@@ -811,7 +812,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     int rank, nrank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
-    const int h = blockIdx.y, g = a.group;
+    const int unit = blockIdx.x / nrank, h = unit % a.n_kv_head, g = a.group;
     const unsigned bar0 = (unsigned) __cvta_generic_to_shared(bars);
     auto full = [&](int s) { return bar0 + 8 * s; };
     auto empty = [&](int s) { return bar0 + 8 * (R + s); };
@@ -823,7 +824,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     if (PARTIAL) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
         PgTile t{};
-        const bool have = pg_find_tile<PARTIAL>(a, blockIdx.x / nrank, t);
+        const bool have = pg_find_tile<PARTIAL>(a, (int) (gridDim.x / nrank) / a.n_kv_head - 1 - unit / a.n_kv_head, t);
         if (lane == 0) { s_have = have; s_tile = t; s_bad = 0; }
     }
     if (tid == 32) {
@@ -1392,13 +1393,14 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     const int64_t parts = PARTIAL ? p.n_prefix : p.n, rows = PARTIAL ? p.n : p.rows;
     const int64_t tiles = std::min((rows * p.group + PT_ROWS - 1) / PT_ROWS + parts, rows * p.group);
     const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
+    if (tiles * p.n_kv_head > (1 << 27)) return cudaErrorInvalidConfiguration;
     int c = 1;
     while (c < 8 && tiles * p.n_kv_head * 2 * c <= 148 && keys > (int64_t) 2 * PT_BN * c) c *= 2;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned) c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned) (tiles * c), (unsigned) p.n_kv_head); cfg.blockDim = dim3(PT_THREADS);
+    cfg.gridDim = dim3((unsigned) (tiles * c * p.n_kv_head)); cfg.blockDim = dim3(PT_THREADS);
     cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
     CUtensorMap mk, mv;
     if (!pg_map(&mk, a.cache.k, a.cache) || !pg_map(&mv, a.cache.v, a.cache)) return cudaErrorInvalidValue;
