@@ -339,6 +339,18 @@ __device__ __forceinline__ float pg_dsm(const float * p, unsigned rank) {
     return v;
 }
 
+// four floats like that, 16-byte aligned
+__device__ __forceinline__ void pg_dsm4(float (&v)[4], const float * p, unsigned rank) {
+    unsigned a = (unsigned) __cvta_generic_to_shared(p), r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(r) : "memory");
+}
+// four values, rounded to the row's type, in one store
+__device__ __forceinline__ void pg_store4(float * p, const float (&v)[4]) { *(float4 *) p = make_float4(v[0], v[1], v[2], v[3]); }
+template <class T> __device__ __forceinline__ void pg_store4(T * p, const float (&v)[4]) {
+    *(uint2 *) p = make_uint2(pg_pack2<T>(v[0], v[1]), pg_pack2<T>(v[2], v[3]));
+}
+
 __host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? 4 : 3; }
 __host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D) * 2 * PD_TK * D * 2; }
 
@@ -656,7 +668,7 @@ __host__ __device__ constexpr int pt_slots(int D, bool f32) { return D == 128 &&
 __host__ __device__ constexpr int pt_q_bytes(int D, bool f32) { return 2 * (f32 ? 2 : 1) * (D / 64) * PT_PANEL; }
 __host__ __device__ constexpr int pt_ring_bytes(int D, bool f32) { return pt_slots(D, f32) * (D / 64) * PT_PANEL; }
 __host__ __device__ constexpr int pt_smem(int D, bool f32) {
-    // the epilogue puts [256][D + 4] floats and two per row over Q and the ring, which are larger
+    // the epilogue's arrays lie over Q and the ring, which are larger
     return 1024 + pt_q_bytes(D, f32) + pt_ring_bytes(D, f32);
 }
 
@@ -783,7 +795,8 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     return false;
 }
 
-static_assert(pt_smem(64, false) >= 1024 + PT_ROWS * (64 + 6) * 4 && pt_smem(128, false) >= 1024 + PT_ROWS * (128 + 6) * 4, "epilogue");
+__host__ __device__ constexpr int pt_epilogue(int D) { return PT_ROWS * ((D + 4) * 4 + 8 + 8 * 4 + 8 + 1); }
+static_assert(pt_smem(64, false) >= 1024 + pt_epilogue(64) && pt_smem(128, false) >= 1024 + pt_epilogue(128), "epilogue");
 
 // grid = tiles x kv heads x splits, clusters of `splits` CTAs, the last tiles
 // (of a prompt, those with the most keys) first.  PARTIAL: the
@@ -808,7 +821,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     __shared__ PgTile s_tile;
     __shared__ int s_have, s_bad;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    float * so = (float *) sm, * s_m = so + PT_ROWS * (D + 4), * s_l = s_m + PT_ROWS;   // epilogue: over Q and the ring
+    // the epilogue's arrays lie over Q and the ring: O, maxima, sums, the parts' weights, the rows' places, marks
+    float * so = (float *) sm, * s_m = so + PT_ROWS * (D + 4), * s_l = s_m + PT_ROWS, * s_w = s_l + PT_ROWS;
+    long long * s_off = (long long *) (s_w + 8 * PT_ROWS);
+    unsigned char * s_odd = (unsigned char *) (s_off + PT_ROWS);
     int rank, nrank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
@@ -874,15 +890,16 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         if (x < nt) {
             // The warp stages its 32 rows, eight lanes to 64 elements: lane c
             // of a row's eight brings 16 bytes of each panel.
+            constexpr int QB = 16 / (NP * PARTS) < 8 ? 16 / (NP * PARTS) : 8;
             const unsigned qd = smq + x * QTILE;
             const int c = lane & 7;
             const float cs = a.scale * 1.4426950408889634f;
             const unsigned flip = a.scale < 0.0f ? 0x80008000u : 0u;   // a negative scale is folded into q
 #pragma unroll
-            for (int b = 0; b < 8; b += 4) {       // four rows of each lane group in flight
-                float4 v[4][NP][PARTS];            // F32: eight floats, else eight 16-bit values in [0]
+            for (int b = 0; b < 8; b += QB) {      // QB rows of each lane group in flight, 16 loads
+                float4 v[QB][NP][PARTS];           // F32: eight floats, else eight 16-bit values in [0]
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < QB; ++k) {
                     const int rw = (r & ~31) + (b + k) * 4 + (lane >> 3), rq = t.lo + rw;
                     const QT * q = (const QT *) a.q + (long long) (t.row0 + rq / g) * a.q_stride + (h * g + rq % g) * D + c * 8;
 #pragma unroll
@@ -892,7 +909,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
                             v[k][p][y] = rw < cnt ? __ldg((const float4 *) (q + p * 64) + y) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
+                for (int k = 0; k < QB; ++k) {
                     const int rr = ((r & ~31) + (b + k) * 4 + (lane >> 3)) & 127;
                     const unsigned off = rr * 128 + ((c ^ (rr & 7)) << 4);
                     if (F32) {
@@ -1033,6 +1050,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
                     *(uint4 *) (so + r * (D + 4) + c + e) = make_uint4(u[e], u[e + 1], u[e + 2], u[e + 3]);
             }
             s_m[r] = m; s_l[r] = l;
+            const long long qrow = t.row0 + tok;
+            const int head = h * g + row % g;
+            s_off[r] = PARTIAL ? (qrow * a.n_head + head) * (D + 4) : qrow * a.out_stride + (long long) head * D;
+            s_odd[r] = 0;
         }
     } else if (warp == 8) {
         // ---------------- MMA issue ----------------
@@ -1206,51 +1227,67 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     if (s_bad && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_TIMEOUT);
     if (nrank > 1) pg_cluster_sync();
 
-    // join the cluster's parts and write: a warp per row
-    constexpr int E = D / 32;
-    for (int r = rank + nrank * warp; r < cnt; r += nrank * (PT_THREADS / 32)) {
-        float mx = -INFINITY, lv = 0.0f, ov[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) ov[e] = 0.0f;
+    // Join the cluster's parts and write, each CTA an equal share of the rows:
+    // first the parts' weights, a thread per row, then four elements per thread.
+    const int share = (cnt + nrank - 1) / nrank, r_beg = min(cnt, rank * share), r_end = min(cnt, r_beg + share);
+    if (tid < r_end - r_beg) {
+        const int r = r_beg + tid;
+        float mx = -INFINITY, lv = 0.0f;
+        for (int y = 0; y < nrank; ++y) mx = fmaxf(mx, pg_dsm(s_m + r, y));
         for (int y = 0; y < nrank; ++y) {
-            float my, ly, oy[E];
-            if (nrank > 1) {
-                my = pg_dsm(s_m + r, y); ly = pg_dsm(s_l + r, y);
-#pragma unroll
-                for (int e = 0; e < E; ++e) oy[e] = pg_dsm(so + r * (D + 4) + lane * E + e, y);
-            } else {
-                my = s_m[r]; ly = s_l[r];
-#pragma unroll
-                for (int e = 0; e < E; ++e) oy[e] = so[r * (D + 4) + lane * E + e];
-            }
-            const float mn = fmaxf(mx, my);
-            const float c = mx == -INFINITY ? 0.0f : pg_exp2(mx - mn), d = my == -INFINITY ? 0.0f : pg_exp2(my - mn);
-            lv = lv * c + ly * d;
-#pragma unroll
-            for (int e = 0; e < E; ++e) ov[e] = ov[e] * c + oy[e] * d;
-            mx = mn;
+            const float my = pg_dsm(s_m + r, y), w = my == -INFINITY ? 0.0f : pg_exp2(my - mx);
+            s_w[y * PT_ROWS + tid] = w;
+            lv += w * pg_dsm(s_l + r, y);
         }
-        const int row = t.lo + r, tok = row / g, head = h * g + row % g;
         if (PARTIAL) {
-            float * rec = a.part + ((long long) (t.row0 + tok) * a.n_head + head) * (D + 4);
-#pragma unroll
-            for (int e = 0; e < E; ++e) rec[lane * E + e] = ov[e];
-            if (lane == 0) { rec[D] = mx; rec[D + 1] = lv; }
+            a.part[s_off[r] + D] = mx;
+            a.part[s_off[r] + D + 1] = lv;
         } else {
-            bool fine = true;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                ov[e] = lv == 0.0f ? 0.0f : ov[e] / lv;
-                fine = fine && fabsf(ov[e]) < INFINITY;
-            }
-            if (!__all_sync(0xffffffffu, fine))
-                pg_row_slow<QT, CT, D>(a, (const QT *) a.q + (long long) (t.row0 + tok) * a.q_stride + head * D, t.i, px, plen,
-                                       len - add + tok + 1, h, ov);
-            QT * out = (QT *) a.out + (long long) (t.row0 + tok) * a.out_stride + head * D;
-#pragma unroll
-            for (int e = 0; e < E; ++e) out[lane * E + e] = pg_from<QT>(ov[e]);
+            const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
+            for (int y = 0; y < nrank; ++y) s_w[y * PT_ROWS + tid] *= inv;
         }
     }
+    __syncthreads();
+    constexpr int C4 = D / 4;
+    bool odd = false;                              // a value that is not finite
+    for (int x = tid; x < (r_end - r_beg) * C4; x += PT_THREADS) {
+        const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
+        float v[4];
+        if (nrank == 1) {
+            const float w = s_w[rr];
+            const float4 u = *(const float4 *) (so + r * (D + 4) + c);
+            v[0] = u.x * w; v[1] = u.y * w; v[2] = u.z * w; v[3] = u.w * w;
+        } else {
+            v[0] = v[1] = v[2] = v[3] = 0.0f;
+            for (int y = 0; y < nrank; ++y) {
+                const float w = s_w[y * PT_ROWS + rr];
+                float u[4];
+                pg_dsm4(u, so + r * (D + 4) + c, y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = fmaf(w, u[e], v[e]);
+            }
+        }
+        if (PARTIAL) {
+            *(float4 *) (a.part + s_off[r] + c) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            pg_store4((QT *) a.out + s_off[r] + c, v);
+            if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
+                s_odd[rr] = 1;
+                odd = true;
+            }
+        }
+    }
+    if (!PARTIAL && __syncthreads_or(odd))         // those rows again, by their keys one by one
+        for (int rr = warp; rr < r_end - r_beg; rr += PT_THREADS / 32) {
+            if (!s_odd[rr]) continue;
+            const int row = t.lo + r_beg + rr, tok = row / g;
+            float sv[D / 32];
+            pg_row_slow<QT, CT, D>(a, (const QT *) a.q + (long long) (t.row0 + tok) * a.q_stride + (h * g + row % g) * D, t.i, px, plen,
+                                   len - add + tok + 1, h, sv);
+            QT * out = (QT *) a.out + s_off[r_beg + rr] + lane * (D / 32);
+#pragma unroll
+            for (int e = 0; e < D / 32; ++e) out[e] = pg_from<QT>(sv[e]);
+        }
     if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
 }
 
