@@ -208,7 +208,7 @@ struct PgAttn {
     const int * len, * table, * row_start, * prefix_start, * prefix_len, * prefix_table;
     int n, rows, n_head, n_kv_head, group, page_log2, n_pages, max_blocks, n_prefix, prefix_max_blocks;
     float scale;
-    float * part;   // prefix parts of a decode batch: [n][n_head][D + 4] floats, (O, max, sum)
+    float * part;   // own parts of a decode batch with prefixes: [n][n_head][D + 4] floats, (O, max, sum)
 };
 
 // the prefix whose range holds request i, or -1
@@ -366,11 +366,13 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     const int i = blockIdx.z, h = blockIdx.y, rank = blockIdx.x, nrank = gridDim.x, g = a.group;
 
+    if (a.part) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int len = __ldg(a.len + i), px = pg_prefix_of(a, i);
     const int plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
     if (len < 0 || len > (a.max_blocks << a.page_log2) || plen < 0 || plen > (a.prefix_max_blocks << a.page_log2)) {
-        if (a.part) asm volatile("griddepcontrol.wait;" ::: "memory");
         if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
+        if (a.part && rank == 0)                   // a negative sum: the tile kernel leaves the row as it is
+            for (int q = tid; q < g; q += 32 * PD_WARPS) a.part[((long long) i * a.n_head + h * g + q) * (D + 4) + D + 1] = -1.0f;
         return;                                    // the whole cluster: it shares i
     }
     const int np = a.part ? 0 : (plen + PD_TK - 1) / PD_TK, total = np + (len + PD_TK - 1) / PD_TK;
@@ -607,17 +609,12 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         co[x] = ov;
         if (x % D == 0) { cm[q] = mx; cl[q] = lv; }
     }
-    if (a.part) asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix parts are there
     if (nrank > 1) pg_cluster_sync(); else __syncthreads();
-    // join the prefix's part and the cluster's CTAs, each an equal share of the outputs
+    // join the cluster's CTAs, each an equal share of the outputs
     QT * out = (QT *) a.out + (long long) i * a.out_stride + h * g * D;
     for (int x = rank * 32 * PD_WARPS + tid; x < g * D; x += nrank * 32 * PD_WARPS) {
         const int q = x / D;
         float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
-        if (a.part && px >= 0) {
-            const float * rec = a.part + ((long long) i * a.n_head + h * g + q) * (D + 4);
-            mx = __ldcg(rec + D); lv = __ldcg(rec + D + 1); ov = __ldcg(rec + x % D);
-        }
         for (int y = 0; y < nrank; ++y) {
             const float my = pg_dsm(cm + q, y), oy = pg_dsm(co + x, y), ly = pg_dsm(cl + q, y);
             const float mn = fmaxf(mx, my);
@@ -625,7 +622,13 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             ov = ov * c + oy * d; lv = lv * c + ly * d;
             mx = mn;
         }
-        out[x] = pg_from<QT>(lv == 0.0f ? 0.0f : ov / lv);
+        if (a.part && px >= 0) {                   // the tile kernel adds the prefix's part
+            float * rec = a.part + ((long long) i * a.n_head + h * g + q) * (D + 4);
+            rec[x % D] = ov;
+            if (x % D == 0) { rec[D] = mx; rec[D + 1] = lv; }
+        } else {
+            out[x] = pg_from<QT>(lv == 0.0f ? 0.0f : ov / lv);
+        }
     }
     if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
 }
@@ -795,13 +798,14 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     return false;
 }
 
-__host__ __device__ constexpr int pt_epilogue(int D) { return PT_ROWS * ((D + 4) * 4 + 8 + 8 * 4 + 8 + 1); }
+__host__ __device__ constexpr int pt_epilogue(int D) { return PT_ROWS * ((D + 4) * 4 + 8 + 8 * 4 + 4 + 16 + 1); }
 static_assert(pt_smem(64, false) >= 1024 + pt_epilogue(64) && pt_smem(128, false) >= 1024 + pt_epilogue(128), "epilogue");
 
 // grid = tiles x kv heads x splits, clusters of `splits` CTAs, the last tiles
 // (of a prompt, those with the most keys) first.  PARTIAL: the
-// prefix keys for all of a decode batch's rows, (O, max, sum) to the
-// workspace; otherwise a prompt's rows, prefix and own keys, to `out`.
+// prefix keys for all of a decode batch's rows, joined with the own parts that
+// the decode kernel left in the workspace; otherwise a prompt's rows over
+// prefix and own keys.
 template <class QT, class CT, int D, bool PARTIAL>
 __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const __grid_constant__ CUtensorMap mk,
                                                                          const __grid_constant__ CUtensorMap mv, PgAttn a) {
@@ -821,10 +825,12 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     __shared__ PgTile s_tile;
     __shared__ int s_have, s_bad;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // the epilogue's arrays lie over Q and the ring: O, maxima, sums, the parts' weights, the rows' places, marks
+    // the epilogue's arrays lie over Q and the ring: O, maxima, sums, the parts' weights, the rows' places in out and
+    // in the own parts, marks
     float * so = (float *) sm, * s_m = so + PT_ROWS * (D + 4), * s_l = s_m + PT_ROWS, * s_w = s_l + PT_ROWS;
-    long long * s_off = (long long *) (s_w + 8 * PT_ROWS);
-    unsigned char * s_odd = (unsigned char *) (s_off + PT_ROWS);
+    float * s_wo = s_w + 8 * PT_ROWS;
+    long long * s_off = (long long *) (s_wo + PT_ROWS), * s_rec = s_off + PT_ROWS;
+    unsigned char * s_odd = (unsigned char *) (s_rec + PT_ROWS);
     int rank, nrank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
@@ -837,7 +843,6 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     auto p_half = [&](int t) { return bar0 + 8 * (2 * R + 4 + t); };
     const unsigned q_full = bar0 + 8 * (2 * R + 6), o_full = bar0 + 8 * (2 * R + 7);
 
-    if (PARTIAL) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
         PgTile t{};
         const bool have = pg_find_tile<PARTIAL>(a, (int) (gridDim.x / nrank) / a.n_kv_head - 1 - unit / a.n_kv_head, t);
@@ -1052,7 +1057,8 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             s_m[r] = m; s_l[r] = l;
             const long long qrow = t.row0 + tok;
             const int head = h * g + row % g;
-            s_off[r] = PARTIAL ? (qrow * a.n_head + head) * (D + 4) : qrow * a.out_stride + (long long) head * D;
+            s_off[r] = qrow * a.out_stride + (long long) head * D;
+            if (PARTIAL) s_rec[r] = (qrow * a.n_head + head) * (D + 4);
             s_odd[r] = 0;
         }
     } else if (warp == 8) {
@@ -1227,29 +1233,32 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     if (s_bad && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_TIMEOUT);
     if (nrank > 1) pg_cluster_sync();
 
-    // Join the cluster's parts and write, each CTA an equal share of the rows:
-    // first the parts' weights, a thread per row, then four elements per thread.
+    // Join the cluster's parts (and a decode row's own part) and write, each
+    // CTA an equal share of the rows: first the parts' weights, a thread per
+    // row, then four elements per thread.
     const int share = (cnt + nrank - 1) / nrank, r_beg = min(cnt, rank * share), r_end = min(cnt, r_beg + share);
+    if (PARTIAL) asm volatile("griddepcontrol.wait;" ::: "memory");   // the own parts are there
     if (tid < r_end - r_beg) {
         const int r = r_beg + tid;
-        float mx = -INFINITY, lv = 0.0f;
+        float mo = -INFINITY, lo = 0.0f;
+        if (PARTIAL) { mo = __ldcg(a.part + s_rec[r] + D); lo = __ldcg(a.part + s_rec[r] + D + 1); }
+        float mx = mo, lv = 0.0f;
         for (int y = 0; y < nrank; ++y) mx = fmaxf(mx, pg_dsm(s_m + r, y));
         for (int y = 0; y < nrank; ++y) {
             const float my = pg_dsm(s_m + r, y), w = my == -INFINITY ? 0.0f : pg_exp2(my - mx);
             s_w[y * PT_ROWS + tid] = w;
             lv += w * pg_dsm(s_l + r, y);
         }
-        if (PARTIAL) {
-            a.part[s_off[r] + D] = mx;
-            a.part[s_off[r] + D + 1] = lv;
-        } else {
-            const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
-            for (int y = 0; y < nrank; ++y) s_w[y * PT_ROWS + tid] *= inv;
-        }
+        const float wo = mo == -INFINITY ? 0.0f : pg_exp2(mo - mx);
+        lv += wo * lo;
+        const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
+        for (int y = 0; y < nrank; ++y) s_w[y * PT_ROWS + tid] *= inv;
+        if (PARTIAL) s_wo[tid] = lo < 0.0f ? -1.0f : wo * inv;        // -1: the request is refused
     }
     __syncthreads();
     constexpr int C4 = D / 4;
     bool odd = false;                              // a value that is not finite
+#pragma unroll 4
     for (int x = tid; x < (r_end - r_beg) * C4; x += PT_THREADS) {
         const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
         float v[4];
@@ -1268,7 +1277,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             }
         }
         if (PARTIAL) {
-            *(float4 *) (a.part + s_off[r] + c) = make_float4(v[0], v[1], v[2], v[3]);
+            const float w = s_wo[rr];
+            const float4 u = __ldcg((const float4 *) (a.part + s_rec[r] + c));
+            if (w > 0.0f) { v[0] = fmaf(w, u.x, v[0]); v[1] = fmaf(w, u.y, v[1]); v[2] = fmaf(w, u.z, v[2]); v[3] = fmaf(w, u.w, v[3]); }
+            if (w != -1.0f) pg_store4((QT *) a.out + s_off[r] + c, v);
         } else {
             pg_store4((QT *) a.out + s_off[r] + c, v);
             if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
@@ -1396,13 +1408,11 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     if (e != cudaSuccess) return e;
     const unsigned c = (unsigned) pg_splits(a);
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[2];
+    cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // runs beside the tile kernel that comes before it
-    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(c, (unsigned) p.n_kv_head, (unsigned) p.n); cfg.blockDim = dim3(32 * PD_WARPS);
-    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = p.part ? 2 : 1;
+    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
 }
 
@@ -1428,17 +1438,19 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     if (e != cudaSuccess) return e;
     // each request (prefix) may end in a part-filled tile
     const int64_t parts = PARTIAL ? p.n_prefix : p.n, rows = PARTIAL ? p.n : p.rows;
-    const int64_t tiles = std::min((rows * p.group + PT_ROWS - 1) / PT_ROWS + parts, rows * p.group);
+    const int64_t tiles = std::min((rows * p.group + PT_ROWS - 1) / PT_ROWS + parts - 1, rows * p.group);
     const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     if (tiles * p.n_kv_head > (1 << 27)) return cudaErrorInvalidConfiguration;
     int c = 1;
     while (c < 8 && tiles * p.n_kv_head * 2 * c <= 148 && keys > (int64_t) 2 * PT_BN * c) c *= 2;
     cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned) c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned) (tiles * c * p.n_kv_head)); cfg.blockDim = dim3(PT_THREADS);
-    cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = PARTIAL ? 2 : 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // PARTIAL: starts as the decode kernel's last CTAs run
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     CUtensorMap mk, mv;
     if (!pg_map(&mk, a.cache.k, a.cache) || !pg_map(&mv, a.cache.v, a.cache)) return cudaErrorInvalidValue;
     return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL>, mk, mv, p);
@@ -1447,13 +1459,10 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
 template <class QT, class CT, int D>
 cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, bool prompt, cudaStream_t st) {
     if (!prompt) {
-        if (p.part) {
-            const cudaError_t e = pg_launch_tiles<QT, CT, D, true>(a, p, st);
-            if (e != cudaSuccess) return e;
-        }
         // F32 queries take two of an M tile's 16 rows
-        if (sizeof(QT) == 4 && p.group > 8) return pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st);
-        return pg_launch_decode<QT, CT, D, 1>(a, p, st);
+        const cudaError_t e = sizeof(QT) == 4 && p.group > 8 ? pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st)
+                                                             : pg_launch_decode<QT, CT, D, 1>(a, p, st);
+        return e != cudaSuccess || !p.part ? e : pg_launch_tiles<QT, CT, D, true>(a, p, st);
     }
     return pg_launch_tiles<QT, CT, D, false>(a, p, st);
 }
