@@ -265,7 +265,13 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 // S = Q K^T comes out in the layout in which P enters P V, so the softmax
 // stays in registers.  F32 queries take two rows, hi and lo, of 11 bits each
 // (K and V are exact in f16), and so do their probabilities.
+#ifndef PD_WARPS
 #define PD_WARPS 4
+#endif
+#ifndef PD_NS64
+#define PD_NS64 3
+#define PD_NS128 2
+#endif
 #define PD_TK 16                // keys of a tile
 #define PD_LAZY 8.0f            // a row is rescaled when its maximum grew by 2^8 or more
 
@@ -351,7 +357,7 @@ template <class T> __device__ __forceinline__ void pg_store4(T * p, const float 
     *(uint2 *) p = make_uint2(pg_pack2<T>(v[0], v[1]), pg_pack2<T>(v[2], v[3]));
 }
 
-__host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? 4 : 3; }
+__host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? PD_NS64 : PD_NS128; }
 __host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D) * 2 * PD_TK * D * 2; }
 
 // grid = (splits, n_kv_head, n), clusters of `splits` CTAs, 128 threads
@@ -367,8 +373,27 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
     const int i = blockIdx.z, h = blockIdx.y, rank = blockIdx.x, nrank = gridDim.x, g = a.group;
 
     if (a.part) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int len = __ldg(a.len + i), px = pg_prefix_of(a, i);
-    const int plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
+    // One trip to memory for the length, the prefix (up to 32 of them) and,
+    // where the tile kernel has the prefix and no cluster splits the keys, the
+    // pages of the warp's first tiles; another for the first keys.
+    const int len = __ldg(a.len + i);
+    int px = -1, plen = 0, early = -1;
+    const bool first = nrank == 1 && (a.part || a.n_prefix == 0);
+    if (first) {
+        const int blk = ((w + (lane >> 1) * PD_WARPS) * PD_TK + (lane & 1) * 8) >> a.page_log2;
+        if (blk < a.max_blocks) early = __ldg(a.table + (long long) i * a.max_blocks + blk);
+    }
+    if (a.n_prefix > 32) {
+        px = pg_prefix_of(a, i);
+        plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
+    } else if (a.n_prefix > 0) {
+        int beg = 0, end = 0, pl = 0;
+        if (lane < a.n_prefix) {
+            beg = __ldg(a.prefix_start + lane); end = __ldg(a.prefix_start + lane + 1); pl = __ldg(a.prefix_len + lane);
+        }
+        px = __ffs(__ballot_sync(0xffffffffu, beg <= i && i < end)) - 1;
+        plen = px >= 0 ? __shfl_sync(0xffffffffu, pl, px) : 0;
+    }
     if (len < 0 || len > (a.max_blocks << a.page_log2) || plen < 0 || plen > (a.prefix_max_blocks << a.page_log2)) {
         if (tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
         if (a.part && rank == 0)                   // a negative sum: the tile kernel leaves the row as it is
@@ -381,7 +406,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 
     // page ids of the warp's next 16 tiles, one per lane and 8-key half: tile
     // x's halves are lanes 2 (x % 16) and 2 (x % 16) + 1; -1 where no key is
-    auto fetch_ids = [&](int x0) {
+    auto fetch_ids = [&](int x0, bool have) {
         const int x = x0 + (lane >> 1);
         int id = -1;
         if (x < mine) {
@@ -389,14 +414,15 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             const bool pre = t < np;
             const int key = (pre ? t : t - np) * PD_TK + (lane & 1) * 8;
             if (key < (pre ? plen : len)) {
-                id = __ldg((pre ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) i * a.max_blocks) +
-                           (key >> a.page_log2));
+                id = have ? early
+                          : __ldg((pre ? a.prefix_table + (long long) px * a.prefix_max_blocks : a.table + (long long) i * a.max_blocks) +
+                                  (key >> a.page_log2));
                 if ((unsigned) id >= (unsigned) a.n_pages) { atomicOr(&g_paged_err, T3B_DEVERR_PAGE); id = -1; }
             }
         }
         return id;
     };
-    int ids = fetch_ids(0), ids_next = -1;
+    int ids = fetch_ids(0, first), ids_next = -1;
 
     const unsigned ring = (unsigned) __cvta_generic_to_shared(pd_sm) + w * NS * 2 * TILE;
     // keys that tile x's half holds (0 .. 8)
@@ -483,7 +509,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
     for (int x = 0; x < mine; ++x) {
         // stage x + NS - 1 is the one that tile x - 1 has left; its ids may be of the next batch
         const int xn = x + NS - 1;
-        if ((x & 15) == 0) ids_next = fetch_ids(x + 16);
+        if ((x & 15) == 0) ids_next = fetch_ids(x + 16, false);
         issue(xn, (xn >> 4) == (x >> 4) ? ids : ids_next);
         asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
         __syncwarp();
@@ -1242,53 +1268,69 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         const int r = r_beg + tid;
         float mo = -INFINITY, lo = 0.0f;
         if (PARTIAL) { mo = __ldcg(a.part + s_rec[r] + D); lo = __ldcg(a.part + s_rec[r] + D + 1); }
-        float mx = mo, lv = 0.0f;
-        for (int y = 0; y < nrank; ++y) mx = fmaxf(mx, pg_dsm(s_m + r, y));
-        for (int y = 0; y < nrank; ++y) {
-            const float my = pg_dsm(s_m + r, y), w = my == -INFINITY ? 0.0f : pg_exp2(my - mx);
-            s_w[y * PT_ROWS + tid] = w;
-            lv += w * pg_dsm(s_l + r, y);
+        float mx = mo, lv = 0.0f, my[8], ly[8];    // every CTA's in flight at once
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            my[y] = y < nrank ? pg_dsm(s_m + r, y) : -INFINITY;
+            ly[y] = y < nrank ? pg_dsm(s_l + r, y) : 0.0f;
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx = fmaxf(mx, my[y]);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            my[y] = my[y] == -INFINITY ? 0.0f : pg_exp2(my[y] - mx);
+            lv += my[y] * ly[y];
         }
         const float wo = mo == -INFINITY ? 0.0f : pg_exp2(mo - mx);
         lv += wo * lo;
         const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
-        for (int y = 0; y < nrank; ++y) s_w[y * PT_ROWS + tid] *= inv;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) if (y < nrank) s_w[y * PT_ROWS + tid] = my[y] * inv;
         if (PARTIAL) s_wo[tid] = lo < 0.0f ? -1.0f : wo * inv;        // -1: the request is refused
     }
     __syncthreads();
     constexpr int C4 = D / 4;
     bool odd = false;                              // a value that is not finite
-#pragma unroll 4
-    for (int x = tid; x < (r_end - r_beg) * C4; x += PT_THREADS) {
-        const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
-        float v[4];
-        if (nrank == 1) {
-            const float w = s_w[rr];
-            const float4 u = *(const float4 *) (so + r * (D + 4) + c);
-            v[0] = u.x * w; v[1] = u.y * w; v[2] = u.z * w; v[3] = u.w * w;
-        } else {
-            v[0] = v[1] = v[2] = v[3] = 0.0f;
-            for (int y = 0; y < nrank; ++y) {
-                const float w = s_w[y * PT_ROWS + rr];
-                float u[4];
-                pg_dsm4(u, so + r * (D + 4) + c, y);
+    auto pieces = [&](auto ranks) {                // the parts' number at compile time: their loads in flight at once
+        constexpr int N = decltype(ranks)::value;
+#pragma unroll(N <= 2 ? 4 : 1)
+        for (int x = tid; x < (r_end - r_beg) * C4; x += PT_THREADS) {
+            const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
+            float v[4], u[N][4];
+            float4 own;
+            if (PARTIAL) own = __ldcg((const float4 *) (a.part + s_rec[r] + c));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = fmaf(w, u[e], v[e]);
+            for (int y = 0; y < N; ++y) {
+                if (N == 1) {
+                    const float4 f = *(const float4 *) (so + r * (D + 4) + c);
+                    u[y][0] = f.x; u[y][1] = f.y; u[y][2] = f.z; u[y][3] = f.w;
+                } else {
+                    pg_dsm4(u[y], so + r * (D + 4) + c, y);
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < N; ++y) {
+                const float w = s_w[y * PT_ROWS + rr];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = y ? fmaf(w, u[y][e], v[e]) : w * u[y][e];
+            }
+            if (PARTIAL) {
+                const float w = s_wo[rr];
+                if (w > 0.0f) { v[0] = fmaf(w, own.x, v[0]); v[1] = fmaf(w, own.y, v[1]); v[2] = fmaf(w, own.z, v[2]); v[3] = fmaf(w, own.w, v[3]); }
+                if (w != -1.0f) pg_store4((QT *) a.out + s_off[r] + c, v);
+            } else {
+                pg_store4((QT *) a.out + s_off[r] + c, v);
+                if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
+                    s_odd[rr] = 1;
+                    odd = true;
+                }
             }
         }
-        if (PARTIAL) {
-            const float w = s_wo[rr];
-            const float4 u = __ldcg((const float4 *) (a.part + s_rec[r] + c));
-            if (w > 0.0f) { v[0] = fmaf(w, u.x, v[0]); v[1] = fmaf(w, u.y, v[1]); v[2] = fmaf(w, u.z, v[2]); v[3] = fmaf(w, u.w, v[3]); }
-            if (w != -1.0f) pg_store4((QT *) a.out + s_off[r] + c, v);
-        } else {
-            pg_store4((QT *) a.out + s_off[r] + c, v);
-            if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
-                s_odd[rr] = 1;
-                odd = true;
-            }
-        }
-    }
+    };
+    if (nrank == 1) pieces(std::integral_constant<int, 1>{});
+    else if (nrank == 2) pieces(std::integral_constant<int, 2>{});
+    else if (nrank == 4) pieces(std::integral_constant<int, 4>{});
+    else pieces(std::integral_constant<int, 8>{});
     if (!PARTIAL && __syncthreads_or(odd))         // those rows again, by their keys one by one
         for (int rr = warp; rr < r_end - r_beg; rr += PT_THREADS / 32) {
             if (!s_odd[rr]) continue;
@@ -1393,7 +1435,7 @@ int pg_splits(const t3b_shared_attn & a) {
     const int64_t units = (int64_t) a.n * a.cache.n_kv_head;
     const int64_t keys = ((int64_t) a.max_blocks + (a.n_prefix > 0 && !pg_shares(a) ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     int c = 1;
-    while (c < 8 && units * c < 4 * 148 && keys > (int64_t) 256 * c) c *= 2;
+    while (c < 8 && units * c < (16 / PD_WARPS) * 148 && keys > (int64_t) 64 * PD_WARPS * c) c *= 2;
     return c;
 }
 
@@ -1442,7 +1484,7 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     if (tiles * p.n_kv_head > (1 << 27)) return cudaErrorInvalidConfiguration;
     int c = 1;
-    while (c < 8 && tiles * p.n_kv_head * 2 * c <= 148 && keys > (int64_t) 2 * PT_BN * c) c *= 2;
+    while (c < 8 && tiles * p.n_kv_head * 2 * c <= (c < 4 ? 148 : 64) && ((PARTIAL && c < 4) || keys > (int64_t) 2 * PT_BN * c)) c *= 2;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
