@@ -265,13 +265,7 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 // S = Q K^T comes out in the layout in which P enters P V, so the softmax
 // stays in registers.  F32 queries take two rows, hi and lo, of 11 bits each
 // (K and V are exact in f16), and so do their probabilities.
-#ifndef PD_WARPS
 #define PD_WARPS 4
-#endif
-#ifndef PD_NS64
-#define PD_NS64 3
-#define PD_NS128 2
-#endif
 #define PD_TK 16                // keys of a tile
 #define PD_LAZY 8.0f            // a row is rescaled when its maximum grew by 2^8 or more
 
@@ -357,7 +351,7 @@ template <class T> __device__ __forceinline__ void pg_store4(T * p, const float 
     *(uint2 *) p = make_uint2(pg_pack2<T>(v[0], v[1]), pg_pack2<T>(v[2], v[3]));
 }
 
-__host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? PD_NS64 : PD_NS128; }
+__host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? 3 : 2; }
 __host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D) * 2 * PD_TK * D * 2; }
 
 // grid = (splits, n_kv_head, n), clusters of `splits` CTAs, 128 threads
@@ -687,19 +681,23 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 //
 // Every wait has a limit (TF_SPIN polls); one that runs out ends the loops of
 // its role, the others' waits run out in turn, and the call is reported.
-#define PT_ROWS 256
 #define PT_BN 128
-#define PT_THREADS 384          // warps 0-7 softmax, 8 MMA, 9-11 loaders: three warps a scheduler, 168 registers
 #define PT_LOADERS 3
 #define PT_PANEL (128 * 128)    // bytes of 128 rows x 64 elements
 
-__host__ __device__ constexpr int pt_slots(int D, bool f32) { return D == 128 && f32 ? 3 : 4; }
-__host__ __device__ constexpr int pt_q_bytes(int D, bool f32) { return 2 * (f32 ? 2 : 1) * (D / 64) * PT_PANEL; }
-__host__ __device__ constexpr int pt_ring_bytes(int D, bool f32) { return pt_slots(D, f32) * (D / 64) * PT_PANEL; }
-__host__ __device__ constexpr int pt_smem(int D, bool f32) {
-    // the epilogue's arrays lie over Q and the ring, which are larger
-    return 1024 + pt_q_bytes(D, f32) + pt_ring_bytes(D, f32);
+// NT: 128-row tiles of a CTA.  Warps 0 .. 4 NT - 1 softmax, then the MMA warp
+// and three loaders: 384 threads of 168 registers, or 256 of 128 (two CTAs a
+// SM), of which the softmax warps take 168 and leave the others 88.
+__host__ __device__ constexpr int pt_threads(int NT) { return 128 * NT + 128; }
+__host__ __device__ constexpr int pt_slots(int D, bool f32, int NT) { return NT == 2 ? (D == 128 && f32 ? 3 : 4) : (D == 128 ? 2 : 4); }
+__host__ __device__ constexpr int pt_q_bytes(int D, bool f32, int NT) { return NT * (f32 ? 2 : 1) * (D / 64) * PT_PANEL; }
+// the epilogue's arrays lie over Q and the ring, which are larger
+__host__ __device__ constexpr int pt_epilogue(int D, int NT) { return 128 * NT * ((D + 4) * 4 + 8 + 8 * 4 + 4 + 16 + 1); }
+__host__ __device__ constexpr int pt_smem(int D, bool f32, int NT) {
+    return 1024 + pt_q_bytes(D, f32, NT) + pt_slots(D, f32, NT) * (D / 64) * PT_PANEL;
 }
+static_assert(pt_smem(64, false, 1) >= 1024 + pt_epilogue(64, 1) && pt_smem(128, false, 1) >= 1024 + pt_epilogue(128, 1) &&
+              pt_smem(64, false, 2) >= 1024 + pt_epilogue(64, 2) && pt_smem(128, false, 2) >= 1024 + pt_epilogue(128, 2), "epilogue");
 
 #define PG_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
 #define PG_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
@@ -766,11 +764,11 @@ __device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned b, un
 // the own keys (PARTIAL: none).
 struct PgTile { int i, px, row0, total, lo, plen, len; };
 
-// The z-th 256-row tile over all requests (prompt) or prefixes, found by one
+// The z-th tile of ROWS rows over all requests (prompt) or prefixes, found by one
 // warp; false past the last one.  Requests whose rows are out of range are
 // passed over.  What the tile needs of its request is loaded beside the
 // starts, and up to 32 prefixes beside those: one trip to memory.
-template <bool PARTIAL>
+template <bool PARTIAL, int ROWS>
 __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     const int lane = threadIdx.x & 31, n = PARTIAL ? a.n_prefix : a.n;
     const int * start = PARTIAL ? a.prefix_start : a.row_start;
@@ -791,7 +789,7 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
                 cnt = 0;
             }
         }
-        const int mine = (int) (((long long) cnt * a.group + PT_ROWS - 1) / PT_ROWS);
+        const int mine = (int) (((long long) cnt * a.group + ROWS - 1) / ROWS);
         int inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -804,7 +802,7 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
             t.i = t.px = b + l;
             t.row0 = __shfl_sync(0xffffffffu, beg, l);
             t.total = __shfl_sync(0xffffffffu, cnt, l) * a.group;
-            t.lo = (z - before - __shfl_sync(0xffffffffu, inc - mine, l)) * PT_ROWS;
+            t.lo = (z - before - __shfl_sync(0xffffffffu, inc - mine, l)) * ROWS;
             t.len = t.plen = __shfl_sync(0xffffffffu, ln, l);
             if (PARTIAL) {
                 t.len = 0;
@@ -824,19 +822,17 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     return false;
 }
 
-__host__ __device__ constexpr int pt_epilogue(int D) { return PT_ROWS * ((D + 4) * 4 + 8 + 8 * 4 + 4 + 16 + 1); }
-static_assert(pt_smem(64, false) >= 1024 + pt_epilogue(64) && pt_smem(128, false) >= 1024 + pt_epilogue(128), "epilogue");
-
 // grid = tiles x kv heads x splits, clusters of `splits` CTAs, the last tiles
 // (of a prompt, those with the most keys) first.  PARTIAL: the
 // prefix keys for all of a decode batch's rows, joined with the own parts that
 // the decode kernel left in the workspace; otherwise a prompt's rows over
 // prefix and own keys.
-template <class QT, class CT, int D, bool PARTIAL>
-__global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const __grid_constant__ CUtensorMap mk,
+template <class QT, class CT, int D, bool PARTIAL, int NT>
+__global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kernel(const __grid_constant__ CUtensorMap mk,
                                                                          const __grid_constant__ CUtensorMap mv, PgAttn a) {
     constexpr bool F32 = sizeof(QT) == 4;
-    constexpr int NP = D / 64, R = pt_slots(D, F32), PARTS = F32 ? 2 : 1;
+    constexpr int NP = D / 64, R = pt_slots(D, F32, NT), PARTS = F32 ? 2 : 1;
+    constexpr int ROWS = 128 * NT, THREADS = pt_threads(NT), MMAW = 4 * NT;   // rows, threads, the MMA warp
     constexpr int SLOT = NP * PT_PANEL, QTILE = PARTS * SLOT;     // bytes
     constexpr float BIAS = PgBias<CT>::v;
     constexpr unsigned FMT = std::is_same<CT, __half>::value ? 0u : (1u << 7) | (1u << 10);
@@ -844,7 +840,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     constexpr unsigned ID_PV = (1u << 4) | FMT | (1u << 16) | ((unsigned) (D >> 3) << 17) | (8u << 24);   // B is MN-major
     extern __shared__ __align__(16) unsigned char pt_raw[];
     unsigned char * sm = pt_raw + ((1024u - ((unsigned) __cvta_generic_to_shared(pt_raw) & 1023u)) & 1023u);
-    const unsigned smq = (unsigned) __cvta_generic_to_shared(sm), smr = smq + 2 * QTILE;
+    const unsigned smq = (unsigned) __cvta_generic_to_shared(sm), smr = smq + NT * QTILE;
     __shared__ __align__(8) unsigned long long bars[2 * R + 8];
     __shared__ __align__(16) unsigned char s_mask[4][16];      // keys present in 8-key groups, of the last four tiles
     __shared__ unsigned s_tmem;
@@ -853,10 +849,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // the epilogue's arrays lie over Q and the ring: O, maxima, sums, the parts' weights, the rows' places in out and
     // in the own parts, marks
-    float * so = (float *) sm, * s_m = so + PT_ROWS * (D + 4), * s_l = s_m + PT_ROWS, * s_w = s_l + PT_ROWS;
-    float * s_wo = s_w + 8 * PT_ROWS;
-    long long * s_off = (long long *) (s_wo + PT_ROWS), * s_rec = s_off + PT_ROWS;
-    unsigned char * s_odd = (unsigned char *) (s_rec + PT_ROWS);
+    float * so = (float *) sm, * s_m = so + ROWS * (D + 4), * s_l = s_m + ROWS, * s_w = s_l + ROWS;
+    float * s_wo = s_w + 8 * ROWS;
+    long long * s_off = (long long *) (s_wo + ROWS), * s_rec = s_off + ROWS;
+    unsigned char * s_odd = (unsigned char *) (s_rec + ROWS);
     int rank, nrank;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(nrank));
@@ -871,7 +867,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
 
     if (warp == 0) {
         PgTile t{};
-        const bool have = pg_find_tile<PARTIAL>(a, (int) (gridDim.x / nrank) / a.n_kv_head - 1 - unit / a.n_kv_head, t);
+        const bool have = pg_find_tile<PARTIAL, ROWS>(a, (int) (gridDim.x / nrank) / a.n_kv_head - 1 - unit / a.n_kv_head, t);
         if (lane == 0) { s_have = have; s_tile = t; s_bad = 0; }
     }
     if (tid == 32) {
@@ -884,37 +880,38 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(p_full(t)) : "memory");
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 128;" ::"r"(p_half(t)) : "memory");
         }
-        asm volatile("mbarrier.init.shared::cta.b64 [%0], 256;" ::"r"(q_full) : "memory");
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(q_full), "n"(ROWS) : "memory");
         asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(o_full) : "memory");
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
-                     ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)) : "memory");
+    if (warp == MMAW) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)), "n"(256 * NT) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 256 + D x
+    const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 128 NT + D x
     const PgTile t = s_tile;
     const int px = t.px, plen = t.plen, len = t.len, add = t.total / g;
     const bool wrong = plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
                        (!PARTIAL && (len < 0 || len > (a.max_blocks << a.page_log2) || add > len));
     if (!s_have || wrong) {                        // the whole cluster: it shares the tile
         if (s_have && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);   // PARTIAL: the decode kernel leaves these requests alone too
-        if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+        if (warp == MMAW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(256 * NT) : "memory");
         return;
     }
-    const int cnt = min(PT_ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
+    const int cnt = min(ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
     // own keys that the tile's last row sees, key tiles of this CTA
     const int seen = PARTIAL ? 0 : len - add + (t.lo + cnt - 1) / g + 1;
     const int np = (plen + PT_BN - 1) / PT_BN, all = np + (seen + PT_BN - 1) / PT_BN;
     const int per = (all + nrank - 1) / nrank, kt0 = min(all, rank * per), nk = min(all, kt0 + per) - kt0;
 
-    if (warp < 8) {
+    if (warp < MMAW) {
         // ---------------- softmax: thread = row ----------------
-        const int x = warp >> 2, r = tid & 255, row = t.lo + r;   // tile, row of the CTA, row of the request
+        if (NT == 1) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        const int x = warp >> 2, r = tid, row = t.lo + r;   // tile, row of the CTA, row of the request
         const int tok = row / g;
         const float sl2 = fabsf(a.scale) * 1.4426950408889634f;
         float sc = sl2;                            // what the row's scores are multiplied by
@@ -985,7 +982,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
 
         float m = -INFINITY, l = 0.0f;
         bool ok = true;
-        const unsigned lanes = tm + ((unsigned) ((warp & 3) * 32) << 16), ts = lanes + 128 * x, to = lanes + 256 + D * x;
+        const unsigned lanes = tm + ((unsigned) ((warp & 3) * 32) << 16), ts = lanes + 128 * x, to = lanes + 128 * NT + D * x;
         const int lim_own = PARTIAL ? 0 : len - add + tok + 1;      // own keys that this row sees
         if (x < nt) {
             for (int j = 0; j < nk; ++j) {
@@ -1064,7 +1061,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         if (!ok) s_bad = 1;
         // (O, max, sum) of the row into shared memory, over Q and the ring:
         // o_full means that every MMA of the CTA has read them
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        asm volatile("bar.sync 1, %0;" ::"n"(ROWS) : "memory");
         if (x < nt) {
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
@@ -1087,7 +1084,10 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             if (PARTIAL) s_rec[r] = (qrow * a.n_head + head) * (D + 4);
             s_odd[r] = 0;
         }
-    } else if (warp == 8) {
+        if (NT == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+    } else {
+    if (NT == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == MMAW) {
         // ---------------- MMA issue ----------------
         const unsigned el = pg_elect();
         // 14 bits of address: in a cluster, shared addresses carry the CTA's rank above them
@@ -1110,7 +1110,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
 #pragma unroll
                 for (int part = 0; part < PARTS; ++part)
-                    pg_mma_ts(tm + 256 + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k), va + k * 128,
+                    pg_mma_ts(tm + 128 * NT + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k), va + k * 128,
                               ID_PV, half == 0 && k == 0 && part == 0 ? acc : 1u, el);
         };
         bool ok = tf_wait(q_full, 0u);
@@ -1150,7 +1150,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         __syncwarp();
     } else {
         // ---------------- loaders: every third group of 8 keys per warp ----------------
-        const int lw = warp - 9;
+        const int lw = warp - MMAW - 1;
         const int items = 2 * nk;
         auto tile_keys = [&](int kt, int & key0, int & have) {        // first key of tile kt in its segment, keys from it on
             const bool pre = kt < np;
@@ -1250,11 +1250,16 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             for (int n = max(0, done - R); n < done; ++n) tf_wait(full(n % R), (unsigned) (n / R) & 1u);
         }
     }
+    if (NT == 1) {
+        __syncwarp();
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    }
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 8) {
+    if (warp == MMAW) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(256 * NT) : "memory");
     }
     if (s_bad && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_TIMEOUT);
     if (nrank > 1) pg_cluster_sync();
@@ -1285,7 +1290,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
         lv += wo * lo;
         const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) if (y < nrank) s_w[y * PT_ROWS + tid] = my[y] * inv;
+        for (int y = 0; y < 8; ++y) if (y < nrank) s_w[y * ROWS + tid] = my[y] * inv;
         if (PARTIAL) s_wo[tid] = lo < 0.0f ? -1.0f : wo * inv;        // -1: the request is refused
     }
     __syncthreads();
@@ -1294,7 +1299,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     auto pieces = [&](auto ranks) {                // the parts' number at compile time: their loads in flight at once
         constexpr int N = decltype(ranks)::value;
 #pragma unroll(N <= 2 ? 4 : 1)
-        for (int x = tid; x < (r_end - r_beg) * C4; x += PT_THREADS) {
+        for (int x = tid; x < (r_end - r_beg) * C4; x += THREADS) {
             const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
             float v[4], u[N][4];
             float4 own;
@@ -1310,7 +1315,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
             }
 #pragma unroll
             for (int y = 0; y < N; ++y) {
-                const float w = s_w[y * PT_ROWS + rr];
+                const float w = s_w[y * ROWS + rr];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = y ? fmaf(w, u[y][e], v[e]) : w * u[y][e];
             }
@@ -1332,7 +1337,7 @@ __global__ __launch_bounds__(PT_THREADS, 1) void attn_shared_tile_kernel(const _
     else if (nrank == 4) pieces(std::integral_constant<int, 4>{});
     else pieces(std::integral_constant<int, 8>{});
     if (!PARTIAL && __syncthreads_or(odd))         // those rows again, by their keys one by one
-        for (int rr = warp; rr < r_end - r_beg; rr += PT_THREADS / 32) {
+        for (int rr = warp; rr < r_end - r_beg; rr += THREADS / 32) {
             if (!s_odd[rr]) continue;
             const int row = t.lo + r_beg + rr, tok = row / g;
             float sv[D / 32];
@@ -1402,13 +1407,16 @@ const char * pg_attn_wrong(const t3b_shared_attn & a, bool prompt, bool pointers
 }
 
 // Whether a decode call computes its prefixes' attention once for the batch
-// (the tile kernel, then joined by the decode kernel) or lets every request
-// read its prefix through L2.
+// (the tile kernel after the decode kernel) or lets every request read its
+// prefix through L2.  The tile kernel costs 6 to 8 us; what it saves is the
+// prefix's K and V for all requests but one, at 5 to 8 TB/s.  Measured with own
+// lengths around 300, us without / with it: 16 x 376 keys (25 MB, f32 x 64
+// dimensions) 14 / 17, 32 x 376 (49 MB) 21 / 25 and (bf16, 8 x 128) 27 / 24,
+// 16 x 1000 (66 MB) 19 / 18 and 27 / 20, 128 x 376 (197 MB) 53 / 43 and 61 / 49.
 bool pg_shares(const t3b_shared_attn & a) {
-    if (a.n_prefix == 0) return false;
-    const char * e = getenv("PGS");
-    if (e) return atoi(e);
-    return true;
+    if (a.n_prefix == 0 || a.n <= a.n_prefix) return false;
+    const double token = 4.0 * a.cache.n_kv_head * a.cache.head_dim;
+    return (double) (a.n - a.n_prefix) * a.prefix_max_blocks * a.cache.page_size * token > 48e6;
 }
 
 size_t pg_workspace(const t3b_shared_attn & a, bool prompt) {
@@ -1435,7 +1443,7 @@ int pg_splits(const t3b_shared_attn & a) {
     const int64_t units = (int64_t) a.n * a.cache.n_kv_head;
     const int64_t keys = ((int64_t) a.max_blocks + (a.n_prefix > 0 && !pg_shares(a) ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     int c = 1;
-    while (c < 8 && units * c < (16 / PD_WARPS) * 148 && keys > (int64_t) 64 * PD_WARPS * c) c *= 2;
+    while (c < 8 && units * c < 4 * 148 && keys > (int64_t) 256 * c) c *= 2;
     return c;
 }
 
@@ -1473,14 +1481,14 @@ bool pg_map(CUtensorMap * map, const void * base, const t3b_paged_kv & c) {
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class QT, class CT, int D, bool PARTIAL>
-cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
-    constexpr bool F32 = sizeof(QT) == 4;
-    const cudaError_t e = pg_allow_smem(attn_shared_tile_kernel<QT, CT, D, PARTIAL>, pt_smem(D, F32));
+template <class QT, class CT, int D, bool PARTIAL, int NT>
+cudaError_t pg_launch_tiles_nt(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
+    constexpr int SMEM = pt_smem(D, sizeof(QT) == 4, NT), ROWS = 128 * NT;
+    const cudaError_t e = pg_allow_smem(attn_shared_tile_kernel<QT, CT, D, PARTIAL, NT>, SMEM);
     if (e != cudaSuccess) return e;
     // each request (prefix) may end in a part-filled tile
     const int64_t parts = PARTIAL ? p.n_prefix : p.n, rows = PARTIAL ? p.n : p.rows;
-    const int64_t tiles = std::min((rows * p.group + PT_ROWS - 1) / PT_ROWS + parts - 1, rows * p.group);
+    const int64_t tiles = std::min((rows * p.group + ROWS - 1) / ROWS + parts - 1, rows * p.group);
     const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     if (tiles * p.n_kv_head > (1 << 27)) return cudaErrorInvalidConfiguration;
     int c = 1;
@@ -1489,13 +1497,26 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned) c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned) (tiles * c * p.n_kv_head)); cfg.blockDim = dim3(PT_THREADS);
-    cfg.dynamicSmemBytes = pt_smem(D, F32); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = PARTIAL ? 2 : 1;
+    cfg.gridDim = dim3((unsigned) (tiles * c * p.n_kv_head)); cfg.blockDim = dim3(pt_threads(NT));
+    cfg.dynamicSmemBytes = SMEM; cfg.stream = st; cfg.attrs = at; cfg.numAttrs = PARTIAL ? 2 : 1;
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // PARTIAL: starts as the decode kernel's last CTAs run
     at[1].val.programmaticStreamSerializationAllowed = 1;
     CUtensorMap mk, mv;
     if (!pg_map(&mk, a.cache.k, a.cache) || !pg_map(&mv, a.cache.v, a.cache)) return cudaErrorInvalidValue;
-    return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL>, mk, mv, p);
+    return cudaLaunchKernelEx(&cfg, attn_shared_tile_kernel<QT, CT, D, PARTIAL, NT>, mk, mv, p);
+}
+
+template <class QT, class CT, int D, bool PARTIAL>
+cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
+    // Two tiles a CTA halve the K / V traffic, which is what 128 dimensions ask
+    // for; with 64 the exponentials bound the loop, and two small CTAs an SM
+    // hide each other's first and last steps.  Measured, one tile against two:
+    // 8 chunks of bf16 x 128 dimensions 368 / 337 us, 4 x 2000 rows of f16 x 64
+    // dimensions 196 / 208; with at most 128 rows to a request the second
+    // tile would be empty: 16 text prompts 23 / 34.
+    if (D == 128 && (PARTIAL ? (int64_t) p.n * p.group > (int64_t) 128 * p.n_prefix : (int64_t) p.rows * p.group > (int64_t) 128 * p.n))
+        return pg_launch_tiles_nt<QT, CT, D, PARTIAL, D == 128 ? 2 : 1>(a, p, st);
+    return pg_launch_tiles_nt<QT, CT, D, PARTIAL, 1>(a, p, st);
 }
 
 template <class QT, class CT, int D>
