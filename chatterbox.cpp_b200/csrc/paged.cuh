@@ -675,7 +675,9 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 // * O stays in tensor memory and is rescaled only when a row's maximum has
 //   grown by 2^8 since the last time (as in the decode kernel).
 // * F32 queries are two f16 parts, and so are their probabilities: two MMAs
-//   into one accumulator.
+//   into one accumulator.  The tensor cores' sums are cut off, not rounded, to
+//   32 bits: over 8000 keys in one accumulator that shrank O by 4.4e-6.  So F32
+//   accumulates one key tile at a time, and the softmax threads add the tiles.
 // * The keys of a tile of rows may be split over a cluster (few rows, many
 //   keys); its CTAs join their (O, max, sum) over distributed shared memory.
 //
@@ -689,7 +691,9 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 // and three loaders: 384 threads of 168 registers, or 256 of 128 (two CTAs a
 // SM), of which the softmax warps take 168 and leave the others 88.
 __host__ __device__ constexpr int pt_threads(int NT) { return 128 * NT + 128; }
-__host__ __device__ constexpr int pt_slots(int D, bool f32, int NT) { return NT == 2 ? (D == 128 && f32 ? 3 : 4) : (D == 128 ? 2 : 4); }
+// (F32 x 128 dimensions has no NT = 2 and no room for a second CTA: tensor memory holds O twice, see below)
+__host__ __device__ constexpr int pt_slots(int D, bool f32, int NT) { return NT == 1 && D == 128 && !f32 ? 2 : 4; }
+__host__ __device__ constexpr int pt_tmem(int D, bool f32, int NT) { return NT == 2 || (f32 && D == 128) ? 512 : 256; }
 __host__ __device__ constexpr int pt_q_bytes(int D, bool f32, int NT) { return NT * (f32 ? 2 : 1) * (D / 64) * PT_PANEL; }
 // the epilogue's arrays lie over Q and the ring, which are larger
 __host__ __device__ constexpr int pt_epilogue(int D, int NT) { return 128 * NT * ((D + 4) * 4 + 8 + 8 * 4 + 4 + 16 + 1); }
@@ -833,6 +837,8 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     constexpr bool F32 = sizeof(QT) == 4;
     constexpr int NP = D / 64, R = pt_slots(D, F32, NT), PARTS = F32 ? 2 : 1;
     constexpr int ROWS = 128 * NT, THREADS = pt_threads(NT), MMAW = 4 * NT;   // rows, threads, the MMA warp
+    constexpr int TCOLS = pt_tmem(D, F32, NT);     // columns of tensor memory
+    static_assert(!F32 || NT == 1, "no room for a sum of tiles");
     constexpr int SLOT = NP * PT_PANEL, QTILE = PARTS * SLOT;     // bytes
     constexpr float BIAS = PgBias<CT>::v;
     constexpr unsigned FMT = std::is_same<CT, __half>::value ? 0u : (1u << 7) | (1u << 10);
@@ -886,20 +892,20 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     }
     if (warp == MMAW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)), "n"(256 * NT) : "memory");
+                     ::"r"((unsigned) __cvta_generic_to_shared(&s_tmem)), "n"(TCOLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 128 NT + D x
+    const unsigned tm = s_tmem;                    // S / P of tile x at 128 x, O at 128 NT + D x, F32's sum of tiles behind
     const PgTile t = s_tile;
     const int px = t.px, plen = t.plen, len = t.len, add = t.total / g;
     const bool wrong = plen < 0 || plen > (a.prefix_max_blocks << a.page_log2) ||
                        (!PARTIAL && (len < 0 || len > (a.max_blocks << a.page_log2) || add > len));
     if (!s_have || wrong) {                        // the whole cluster: it shares the tile
         if (s_have && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);   // PARTIAL: the decode kernel leaves these requests alone too
-        if (warp == MMAW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(256 * NT) : "memory");
+        if (warp == MMAW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(TCOLS) : "memory");
         return;
     }
     const int cnt = min(ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
@@ -984,6 +990,12 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
         bool ok = true;
         const unsigned lanes = tm + ((unsigned) ((warp & 3) * 32) << 16), ts = lanes + 128 * x, to = lanes + 128 * NT + D * x;
         const int lim_own = PARTIAL ? 0 : len - add + tok + 1;      // own keys that this row sees
+        if (F32) {                                 // the sum of tiles
+            const unsigned zero[16] = {};
+#pragma unroll
+            for (int c = 0; c < D; c += 16) pg_tm_st16(zero, to + D + c);
+            pg_tm_wait_st();
+        }
         if (x < nt) {
             for (int j = 0; j < nk; ++j) {
                 ok = tf_wait(s_full(x), (unsigned) j & 1u);
@@ -991,6 +1003,17 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const int kt = kt0 + j;
                 const int left = kt < np ? PT_BN : lim_own - (kt - np) * PT_BN;   // keys of the tile before the causal limit
+                if (F32 && j > 0)                  // the last tile's O is complete: add it to the sum
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        unsigned w[16], v[16];
+                        pg_tm_ld16(w, to + c);
+                        pg_tm_ld16(v, to + D + c);
+                        pg_tm_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) + __uint_as_float(v[e]));
+                        pg_tm_st16(w, to + D + c);
+                    }
                 unsigned u[4][32];                 // the row's scores
 #pragma unroll
                 for (int c = 0; c < 4; ++c) pg_tm_ld32(u[c], ts + 32 * c);
@@ -1020,11 +1043,13 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
                             unsigned w[16];
-                            pg_tm_ld16(w, to + c);
+                            const unsigned at = to + (F32 ? D : 0) + c;
+                            if (F32) pg_tm_wait_st();
+                            pg_tm_ld16(w, at);
                             pg_tm_wait_ld();
 #pragma unroll
                             for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
-                            pg_tm_st16(w, to + c);
+                            pg_tm_st16(w, at);
                         }
                 }
                 const float base = m == -INFINITY ? 0.0f : m - BIAS;
@@ -1067,8 +1092,13 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
             for (int c = 0; c < D; c += 32) {
                 unsigned u[32];
                 if (nk > 0) {
+                    unsigned v[32];
                     pg_tm_ld32(u, to + c);
+                    if (F32) pg_tm_ld32(v, to + D + c);
                     pg_tm_wait_ld();
+                    if (F32)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) + __uint_as_float(v[e]));
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) u[e] = 0u;
@@ -1132,7 +1162,7 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
                 ok = tf_wait(p_half(x), (unsigned) j & 1u);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                pv(x, sv, j > 0, 0);
+                pv(x, sv, !F32 && j > 0, 0);
                 ok = tf_wait(p_full(x), (unsigned) j & 1u);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -1259,7 +1289,7 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     __syncthreads();
     if (warp == MMAW) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(256 * NT) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(TCOLS) : "memory");
     }
     if (s_bad && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_TIMEOUT);
     if (nrank > 1) pg_cluster_sync();
@@ -1514,8 +1544,8 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
     // 8 chunks of bf16 x 128 dimensions 368 / 337 us, 4 x 2000 rows of f16 x 64
     // dimensions 196 / 208; with at most 128 rows to a request the second
     // tile would be empty: 16 text prompts 23 / 34.
-    if (D == 128 && (PARTIAL ? (int64_t) p.n * p.group > (int64_t) 128 * p.n_prefix : (int64_t) p.rows * p.group > (int64_t) 128 * p.n))
-        return pg_launch_tiles_nt<QT, CT, D, PARTIAL, D == 128 ? 2 : 1>(a, p, st);
+    if (D == 128 && sizeof(QT) == 2 && (PARTIAL ? (int64_t) p.n * p.group > (int64_t) 128 * p.n_prefix : (int64_t) p.rows * p.group > (int64_t) 128 * p.n))
+        return pg_launch_tiles_nt<QT, CT, D, PARTIAL, D == 128 && sizeof(QT) == 2 ? 2 : 1>(a, p, st);
     return pg_launch_tiles_nt<QT, CT, D, PARTIAL, 1>(a, p, st);
 }
 
