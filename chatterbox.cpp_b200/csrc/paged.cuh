@@ -17,6 +17,7 @@ static __device__ unsigned g_paged_err;
 #define PG_PLAN_T 1024
 #define PG_PLAN_MAXN 8192
 #define PG_PLAN_CLUSTER 8
+#define PG_PLAN_ROWS 16384   // from this many rows on a kernel of its own fills them in
 
 // exclusive prefix sums of two 64-bit values over the CTA; `tot` gets the sums
 __device__ __forceinline__ void pg_scan2(unsigned long long & a, unsigned long long & b, unsigned long long (*red)[2],
@@ -31,7 +32,8 @@ __device__ __forceinline__ void pg_scan2(unsigned long long & a, unsigned long l
     __syncthreads();   // red is reused
     if (lane == 31) { red[w][0] = ia; red[w][1] = ib; }
     __syncthreads();
-    unsigned long long va = red[lane][0], vb = red[lane][1];   // PG_PLAN_T / 32 = 32 warps
+    const bool on = lane < (int) (blockDim.x >> 5);
+    unsigned long long va = on ? red[lane][0] : 0ull, vb = on ? red[lane][1] : 0ull;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long xa = __shfl_up_sync(0xffffffffu, va, o), xb = __shfl_up_sync(0xffffffffu, vb, o);
@@ -54,6 +56,67 @@ __device__ __forceinline__ int pg_find(const int * at, int n, int x) {
     return lo;
 }
 
+// Rows r0 .. r0 + 3 of the row maps: one bisection of s_row (n + 1 first
+// rows) and, mostly, one page id for all four.  start(i): the own tokens
+// before the step; page(i, b): table entry b of request i.
+template <class Start, class Page>
+__device__ __forceinline__ void pg_plan_rows(const t3b_kv_plan & p, int n, int nrow, int lg, int r0, const int * s_row, Start start, Page page) {
+    int req[4], pos[4], slot[4];
+    int i = r0 < nrow ? pg_find(s_row, n, r0) : 0, have = -1, id = -1, ln = r0 < nrow ? start(i) : 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int r = r0 + e;
+        req[e] = pos[e] = slot[e] = -1;
+        if (r >= nrow) continue;
+        if (r >= s_row[i + 1]) {
+            do ++i; while (r >= s_row[i + 1]);
+            ln = start(i);
+            have = -1;
+        }
+        req[e] = i;
+        pos[e] = ln + (r - s_row[i]);
+        const int blk = pos[e] >> lg;
+        if (blk != have) {
+            have = blk;
+            id = page(i, blk);
+            if (id < 0 || id > (0x7fffffff - (1 << lg) + 1) >> lg) {   // the slot would not fit 31 bits
+                atomicOr(&g_paged_err, T3B_DEVERR_PAGE);
+                id = -1;
+            }
+        }
+        if (id >= 0) slot[e] = (id << lg) + (pos[e] & ((1 << lg) - 1));
+    }
+    if (((((uintptr_t) p.row_req) | ((uintptr_t) p.row_pos) | ((uintptr_t) p.slots)) & 15) == 0 && r0 + 4 <= p.rows_cap) {
+        if (p.row_req) *(int4 *) (p.row_req + r0) = make_int4(req[0], req[1], req[2], req[3]);
+        if (p.row_pos) *(int4 *) (p.row_pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        if (p.slots) *(int4 *) (p.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (r0 + e >= p.rows_cap) break;
+            if (p.row_req) p.row_req[r0 + e] = req[e];
+            if (p.row_pos) p.row_pos[r0 + e] = pos[e];
+            if (p.slots) p.slots[r0 + e] = slot[e];
+        }
+    }
+}
+
+// The row maps of a large step, over the whole GPU, from what the plan kernel
+// left: a step of 2048 requests and 200 000 rows took
+// 18 us in one cluster and takes 12 so.
+__global__ __launch_bounds__(256) void kv_plan_rows_kernel(t3b_kv_plan p) {
+    extern __shared__ int pg_sm[];
+    const int n = p.n, lg = __ffs(p.page_size) - 1;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int i = threadIdx.x; i <= n; i += 256) pg_sm[i] = __ldcg(p.row_start + i);
+    __syncthreads();
+    const int r0 = 4 * (blockIdx.x * 256 + threadIdx.x);
+    if (r0 >= p.rows_cap) return;
+    auto start = [&](int i) { return p.len_out ? __ldcg(p.len_out + i) - (pg_sm[i + 1] - pg_sm[i]) : __ldcg(p.len + i); };
+    auto page = [&](int i, int blk) { return __ldcg(p.table + (size_t) i * p.max_blocks + blk); };
+    pg_plan_rows(p, n, pg_sm[n], lg, r0, pg_sm, start, page);
+}
+
 // One cluster.  Every CTA scans all requests (a few KB), so all of them know
 // each request's first row, first new page and first returned page and come
 // to the same verdict; the returned pages, the new pages and the rows are
@@ -62,28 +125,36 @@ __device__ __forceinline__ int pg_find(const int * at, int n, int x) {
 // reads the old state (lengths, n_free, the released rows of the table) from
 // what overwrites it, which is what lets a slot be released and admitted in
 // one step and the outputs be the inputs' own buffers.
-__global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p) {
+__global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p, bool rows_here) {
     extern __shared__ int pg_sm[];
     __shared__ unsigned long long red[32][2];
-    int * s_len = pg_sm, * s_row = s_len + p.n, * s_take = s_row + p.n, * s_back = s_take + p.n;
-    const int tid = threadIdx.x, n = p.n, P = p.page_size;
+    int * s_len = pg_sm, * s_take = s_len + p.n, * s_back = s_take + p.n, * s_row = s_back + p.n;   // s_row: n + 1
+    const int tid = threadIdx.x, T = blockDim.x, n = p.n, P = p.page_size, lg = __ffs(P) - 1;
     unsigned rank, csize;
+    if (!rows_here) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
     const long long cap = (long long) p.max_blocks * P;
     const int F = *p.n_free;
     unsigned long long rows = 0, pages = 0;   // pages: new ones in the low half, returned ones in the high
     int bad = 0;
-    for (int t0 = 0; t0 < n; t0 += PG_PLAN_T) {
+    int ln_next = 0, ad_next = 0, rl_next = 0;
+    if (tid < n) { ln_next = p.len[tid]; ad_next = p.add[tid]; if (p.release) rl_next = p.release[tid]; }
+    for (int t0 = 0; t0 < n; t0 += T) {
         const int i = t0 + tid;
-        int ln = 0, ad = 0, rl = 0;
-        if (i < n) {
-            ln = p.len[i]; ad = p.add[i]; rl = p.release ? p.release[i] : 0;
+        int ln = ln_next, ad = ad_next, rl = rl_next;
+        if (i + T < n) {                   // in flight during this tile's scan
+            ln_next = p.len[i + T]; ad_next = p.add[i + T];
+            if (p.release) rl_next = p.release[i + T];
+        }
+        if (i >= n) {
+            ln = ad = rl = 0;
+        } else {
             if (ln < 0 || ad < 0 || rl < 0 || (long long) ln + ad > cap || rl > cap || (rl > 0 && ln > 0)) {
                 bad = 1; ln = ad = rl = 0;
             }
         }
-        const unsigned take = (unsigned) ((ln + ad + P - 1) / P - (ln + P - 1) / P), back = (unsigned) ((rl + P - 1) / P);
+        const unsigned take = (unsigned) (((ln + ad + P - 1) >> lg) - ((ln + P - 1) >> lg)), back = (unsigned) ((rl + P - 1) >> lg);
         unsigned long long a = (unsigned long long) ad, b = ((unsigned long long) back << 32) | take, ta, tb;
         pg_scan2(a, b, red, ta, tb);
         a += rows; b += pages;
@@ -101,7 +172,8 @@ __global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p) {
     bad = __syncthreads_or(bad);
     const bool ok = !bad && fits && !over;
     const int nrow = ok ? (int) rows : 0;
-    const int me = (int) rank * PG_PLAN_T + tid, all = (int) csize * PG_PLAN_T;
+    if (tid == 0) s_row[n] = nrow;                 // read after the cluster's barrier
+    const int me = (int) rank * T + tid, all = (int) csize * T;
     if (ok)   // returned pages, on top of the stack
         for (int k = me; k < back_n; k += all) {
             const int i = pg_find(s_back, n, k);
@@ -113,28 +185,20 @@ __global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p) {
     if (ok)   // new pages
         for (int k = me; k < take_n; k += all) {
             const int i = pg_find(s_take, n, k);
-            p.table[(size_t) i * p.max_blocks + (s_len[i] + P - 1) / P + (k - s_take[i])] = p.free_pages[top - 1 - k];
+            p.table[(size_t) i * p.max_blocks + ((s_len[i] + P - 1) >> lg) + (k - s_take[i])] = p.free_pages[top - 1 - k];
         }
-    for (int r = me; r < p.rows_cap; r += all) {
-        int req = -1, pos = -1, slot = -1;
-        if (r < nrow) {
-            req = pg_find(s_row, n, r);
-            pos = s_len[req] + (r - s_row[req]);
-            const int blk = pos / P, held = (s_len[req] + P - 1) / P;
-            const int id = blk < held ? p.table[(size_t) req * p.max_blocks + blk]
-                                      : p.free_pages[top - 1 - (s_take[req] + blk - held)];
-            const bool sane = id >= 0 && id <= (0x7fffffff - P + 1) / P;   // the slot fits 31 bits
-            slot = sane ? id * P + pos % P : -1;
-            if (!sane) atomicOr(&g_paged_err, T3B_DEVERR_PAGE);
-        }
-        if (p.row_req) p.row_req[r] = req;
-        if (p.row_pos) p.row_pos[r] = pos;
-        if (p.slots) p.slots[r] = slot;
+    if (rows_here) {
+        auto page = [&](int i, int blk) {
+            const int held = (s_len[i] + P - 1) >> lg;
+            return blk < held ? p.table[(size_t) i * p.max_blocks + blk] : p.free_pages[top - 1 - (s_take[i] + blk - held)];
+        };
+        auto start = [&](int i) { return s_len[i]; };
+        for (int r0 = 4 * me; r0 < p.rows_cap; r0 += 4 * all) pg_plan_rows(p, n, nrow, lg, r0, s_row, start, page);
     }
     for (int i = me; i < n; i += all) {
         p.row_start[i] = ok ? s_row[i] : 0;
         if (p.len_out) {
-            if (ok) p.len_out[i] = s_len[i] + (i + 1 < n ? s_row[i + 1] : nrow) - s_row[i];
+            if (ok) p.len_out[i] = s_len[i] + s_row[i + 1] - s_row[i];
             else if (p.len_out != p.len) p.len_out[i] = p.len[i];
         }
     }
@@ -1591,25 +1655,37 @@ extern "C" {
 int t3b_op_kv_plan(const t3b_kv_plan * p, void * cuda_stream) {
     int lg;
     if (!p || !p->len || !p->add || !p->free_pages || !p->n_free || !p->n_free_out || !p->table || !p->row_start ||
-        p->n <= 0 || p->n > PG_PLAN_MAXN || p->rows_cap < 0 || p->free_cap < 0 || p->max_blocks <= 0 ||
+        p->n <= 0 || p->n > PG_PLAN_MAXN || p->rows_cap < 0 || p->rows_cap > 1 << 30 || p->free_cap < 0 || p->max_blocks <= 0 ||
         !pg_log2(p->page_size, 3, 8, &lg) || (int64_t) p->max_blocks * p->page_size > 0x3fffffffll ||
         (int64_t) p->n * p->max_blocks > 0x3fffffffll) {
         set_err(nullptr, "t3b_op_kv_plan: bad args");
         return T3B_ERR_ARG;
     }
-    const size_t smem = (size_t) 4 * p->n * sizeof(int);
+    const size_t smem = ((size_t) 4 * p->n + 1) * sizeof(int);
     if (smem > 40 * 1024 &&
-        cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * PG_PLAN_MAXN * (int) sizeof(int)) != cudaSuccess) {
+        cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * PG_PLAN_MAXN + 1) * (int) sizeof(int)) != cudaSuccess) {
         set_err(nullptr, "t3b_op_kv_plan: shared memory attribute");
         return T3B_ERR_CUDA;
     }
+    // one CTA does for few requests and rows; eight cost 0.3 us more and take a larger step's work apart
+    const bool rows_here = p->rows_cap <= PG_PLAN_ROWS || (!p->row_req && !p->row_pos && !p->slots);
+    const int most = std::max(p->n, p->rows_cap / 4);
+    const unsigned threads = most <= 128 ? 128 : most <= 256 ? 256 : PG_PLAN_T;
+    const unsigned c = p->n <= PG_PLAN_T && p->rows_cap <= 4096 ? 1 : PG_PLAN_CLUSTER;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = PG_PLAN_CLUSTER; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(PG_PLAN_CLUSTER); cfg.blockDim = dim3(PG_PLAN_T); cfg.dynamicSmemBytes = smem;
+    at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(c); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t) cuda_stream; cfg.attrs = at; cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, *p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, *p, rows_here);
+    if (e == cudaSuccess && !rows_here) {
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.gridDim = dim3((unsigned) ((p->rows_cap + 1023) / 1024)); cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = ((size_t) p->n + 1) * sizeof(int);
+        e = cudaLaunchKernelEx(&cfg, kv_plan_rows_kernel, *p);
+    }
     if (e != cudaSuccess) { set_err(nullptr, "t3b_op_kv_plan: %s", cudaGetErrorString(e)); (void) cudaGetLastError(); return T3B_ERR_CUDA; }
     return T3B_OK;
 }

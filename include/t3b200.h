@@ -378,7 +378,7 @@ typedef struct t3b_paged_kv {
  * rows, release[i] > 0 with len[i] > 0, n_free outside the stack, or no room
  * on it) changes nothing: table and stack stay as they are, n_free_out =
  * n_free, len_out = len, row_start is 0, all rows are -1, and t3b_op_check
- * reports it.  n <= 8192. */
+ * reports it.  n <= 8192, rows_cap <= 2^30. */
 typedef struct t3b_kv_plan {
     int32_t n;               /* requests (slots) */
     int32_t page_size;

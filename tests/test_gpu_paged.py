@@ -115,6 +115,26 @@ def test_plan_matches_its_definition(pkg, n, page, width, readmit):
         _same(p.got(), ref)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("n,page,width,rows_cap", [(700, 16, 9, None), (3000, 8, 8, None), (300, 32, 20, 100003), (5, 256, 40, 40000)])
+def test_plan_of_many_rows(pkg, n, page, width, rows_cap, in_place):
+    """Steps of tens of thousands of rows, with in-place lengths and room to spare."""
+    rng = np.random.default_rng(n)
+    ln, add, release, table, free, n_free = _random_step(rng, n, page, width, True)
+    cap = rows_cap or int(add.sum())
+    assert 16384 < cap and add.sum() <= cap
+    p = Plan(pkg, ln, add, release, page, table, free, n_free, cap, in_place=in_place)
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    _same(p.got(), paged_ref.plan(ln, add, release, page, table, free, n_free, cap))
+    # one page too few: nothing changes, all of the large row maps are -1
+    q = Plan(pkg, ln, add, release, page, table, free, 0, cap, in_place=in_place)
+    if paged_ref.plan(ln, add, release, page, table, free, 0, cap) is None:
+        pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(q.d), _stream()))
+        assert pkg.lib().t3b_op_check(_stream()) == -5
+        got = q.got()
+        assert all((got[k] == -1).all() for k in ("row_req", "row_pos", "slots")) and np.array_equal(got["table"], table)
+
+
 def test_plan_without_the_optional_arrays(pkg):
     rng = np.random.default_rng(5)
     ln, add, _, table, free, n_free = _random_step(rng, 40, 16, 6, False)
