@@ -346,6 +346,9 @@ __device__ __forceinline__ float pg_exp2(float x) {
 __device__ __forceinline__ void pg_cp16(unsigned dst, const void * src, bool on) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void pg_cp16(unsigned dst, const void * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void pg_ldm4(unsigned (&r)[4], unsigned addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -441,6 +444,27 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         const int blk = ((w + (lane >> 1) * PD_WARPS) * PD_TK + (lane & 1) * 8) >> a.page_log2;
         if (blk < a.max_blocks) early = __ldg(a.table + (long long) i * a.max_blocks + blk);
     }
+    unsigned qf[MT][KS][4];                        // queries as A fragments
+    float2 qv[F32 ? MT : 1][KS][2];                // F32: as they come
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            if (F32) {
+                const int r = mt * RPM + (lane >> 2);
+                const float * q = (const float *) a.q + (long long) i * a.q_stride + (h * g + min(r, g - 1)) * D;
+#pragma unroll
+                for (int b = 0; b < 2; ++b) qv[mt][k][b] = *(const float2 *) (q + k * 16 + b * 8 + (lane & 3) * 2);
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const int r = mt * RPM + (lane >> 2) + (b & 1) * 8;
+                    qf[mt][k][b] = r < g ? *(const unsigned *) ((const CT *) a.q + (long long) i * a.q_stride + (h * g + r) * D +
+                                                                k * 16 + (b >> 1) * 8 + (lane & 3) * 2)
+                                         : 0u;
+                }
+            }
+        }
     if (a.n_prefix > 32) {
         px = pg_prefix_of(a, i);
         plen = px >= 0 ? __ldg(a.prefix_len + px) : 0;
@@ -489,48 +513,65 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         const int left = (t < np ? plen - t * PD_TK : len - (t - np) * PD_TK) - half * 8;
         return id < 0 ? 0 : min(8, left);
     };
-    auto issue = [&](int x, int my_ids) {          // tile x's K and V into stage x % NS
+    // lane's chunk of rows (lane / CH) + RPC c: where it lies in an 8-key half
+    constexpr int RPC = 32 / CH, CPH = 8 / RPC;    // rows an instruction moves, instructions a half
+    const int lrow = lane / CH, lch = lane % CH;
+    unsigned spot[CPH];
+#pragma unroll
+    for (int c = 0; c < CPH; ++c) spot[c] = (c * RPC + lrow) * (D * 2) + ((lch ^ (c * RPC + lrow)) << 4);
+    const long long lane_off = (((long long) h << a.page_log2) + lrow) * D + lch * 8;
+    const int mask = (1 << a.page_log2) - 1;
+    auto issue = [&](int x, int my_ids, int slot) {   // tile x's K and V into a stage
         if (x < mine) {
             const int t = t_beg + w + x * PD_WARPS, key0 = (t < np ? t : t - np) * PD_TK;
-            const unsigned st = ring + (x % NS) * 2 * TILE;
+            const unsigned st = ring + slot * 2 * TILE;
+            const int left = (t < np ? plen : len) - key0;
+            int id[2];
+            const CT * kp[2], * vp[2];
 #pragma unroll
-            for (int c = 0; c < PD_TK * CH / 32; ++c) {
-                const int q = lane + c * 32, row = q / CH, ch = q % CH;
-                const int id = __shfl_sync(0xffffffffu, my_ids, 2 * (x & 15) + (row >> 3));
-                const bool on = (row & 7) < half_keys(x, row >> 3, id);
-                const int key = key0 + row;
-                const long long off = on ? (long long) id * a.page_stride +
-                                               (((long long) h << a.page_log2) + (key & ((1 << a.page_log2) - 1))) * D + ch * 8
-                                         : 0;
-                const unsigned d = st + row * (D * 2) + ((ch ^ (row & 7)) << 4);
-                pg_cp16(d, (const CT *) a.k + off, on);
-                pg_cp16(d + TILE, (const CT *) a.v + off, on);   // keys past the end are zeros: 0 * NaN would stay
+            for (int b = 0; b < 2; ++b) {
+                id[b] = __shfl_sync(0xffffffffu, my_ids, 2 * (x & 15) + b);
+                const long long off = (long long) max(id[b], 0) * a.page_stride + ((key0 + 8 * b) & mask) * D + lane_off;
+                kp[b] = (const CT *) a.k + off; vp[b] = (const CT *) a.v + off;
+            }
+            if (left >= PD_TK && (id[0] | id[1]) >= 0) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int c = 0; c < CPH; ++c) {
+                        pg_cp16(st + spot[c] + b * 8 * D * 2, kp[b] + c * RPC * D);
+                        pg_cp16(st + spot[c] + b * 8 * D * 2 + TILE, vp[b] + c * RPC * D);
+                    }
+            } else {                               // keys past the end are zeros: 0 * NaN would stay
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int c = 0; c < CPH; ++c) {
+                        const bool on = id[b] >= 0 && c * RPC + lrow + 8 * b < left;
+                        pg_cp16(st + spot[c] + b * 8 * D * 2, on ? kp[b] + c * RPC * D : (const CT *) a.k, on);
+                        pg_cp16(st + spot[c] + b * 8 * D * 2 + TILE, on ? vp[b] + c * RPC * D : (const CT *) a.v, on);
+                    }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int x = 0; x < NS - 1; ++x) issue(x, ids);
+    for (int x = 0; x < NS - 1; ++x) issue(x, ids, x);
 
-    // queries as A fragments
-    unsigned qf[MT][KS][4];
     float sc[MT][2];                               // what a score of row lane / 4 (+ 8) is multiplied by
     const float sl2 = a.scale * 1.4426950408889634f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         if (F32) {
-            const int r = mt * RPM + (lane >> 2);
-            const float * q = (const float *) a.q + (long long) i * a.q_stride + (h * g + min(r, g - 1)) * D;
-            float2 v[KS][2];
             float mx = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    v[k][b] = *(const float2 *) (q + k * 16 + b * 8 + (lane & 3) * 2);
-                    if (r >= g) v[k][b] = make_float2(0.f, 0.f);
-                    v[k][b].x *= sl2; v[k][b].y *= sl2;
-                    mx = fmaxf(mx, fmaxf(fabsf(v[k][b].x), fabsf(v[k][b].y)));
+                    float2 & v = qv[mt][k][b];
+                    if (mt * RPM + (lane >> 2) >= g) v = make_float2(0.f, 0.f);
+                    v.x *= sl2; v.y *= sl2;
+                    mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -540,18 +581,9 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
-                for (int b = 0; b < 2; ++b) pg_split2(v[k][b].x * f, v[k][b].y * f, qf[mt][k][2 * b], qf[mt][k][2 * b + 1]);
+                for (int b = 0; b < 2; ++b) pg_split2(qv[mt][k][b].x * f, qv[mt][k][b].y * f, qf[mt][k][2 * b], qf[mt][k][2 * b + 1]);
         } else {
             sc[mt][0] = sc[mt][1] = sl2;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int r = mt * RPM + (lane >> 2) + (b & 1) * 8;
-                    qf[mt][k][b] = r < g ? *(const unsigned *) ((const CT *) a.q + (long long) i * a.q_stride + (h * g + r) * D +
-                                                                k * 16 + (b >> 1) * 8 + (lane & 3) * 2)
-                                         : 0u;
-                }
         }
     }
 
@@ -564,16 +596,17 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         for (int d = 0; d < D / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
     }
     const int lr = lane & 7, mi = lane >> 3;       // ldmatrix: row of matrix mi
+    int slot = 0, slot_in = NS - 1;                // stages of tiles x and x + NS - 1
     for (int x = 0; x < mine; ++x) {
         // stage x + NS - 1 is the one that tile x - 1 has left; its ids may be of the next batch
         const int xn = x + NS - 1;
         if ((x & 15) == 0) ids_next = fetch_ids(x + 16, false);
-        issue(xn, (xn >> 4) == (x >> 4) ? ids : ids_next);
+        issue(xn, (xn >> 4) == (x >> 4) ? ids : ids_next, slot_in);
         asm volatile("cp.async.wait_group %0;" ::"n"(NS - 1) : "memory");
         __syncwarp();
         const int n0 = half_keys(x, 0, __shfl_sync(0xffffffffu, ids, 2 * (x & 15)));
         const int n1 = half_keys(x, 1, __shfl_sync(0xffffffffu, ids, 2 * (x & 15) + 1));
-        const unsigned st = ring + (x % NS) * 2 * TILE;
+        const unsigned st = ring + slot * 2 * TILE;
         float s[MT][2][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -650,6 +683,8 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             }
         }
         __syncwarp();
+        if (++slot == NS) slot = 0;
+        if (++slot_in == NS) slot_in = 0;
         if ((x & 15) == 15) ids = ids_next;
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -679,42 +714,64 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             }
         }
     __syncthreads();
-    for (int x = tid; x < g * D; x += 32 * PD_WARPS) {
-        const int q = x / D;
-        float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
+    // four elements a thread; an only CTA writes what it has, a cluster's
+    // share the elements out once each has joined its warps
+    constexpr int D4 = D / 4;
+    QT * out = (QT *) a.out + (long long) i * a.out_stride + h * g * D;
+    float * rec = a.part + ((long long) i * a.n_head + h * g) * (D + 4);
+    auto finish = [&](int q, int c, float mx, float lv, float (&v)[4]) {
+        if (a.part && px >= 0) {                   // the tile kernel adds the prefix's part
+            pg_store4(rec + q * (D + 4) + c, v);
+            if (c == 0) { rec[q * (D + 4) + D] = mx; rec[q * (D + 4) + D + 1] = lv; }
+        } else {
+            const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
 #pragma unroll
-        for (int y = 0; y < PD_WARPS; ++y) mx = fmaxf(mx, sm[y * g + q]);
+            for (int e = 0; e < 4; ++e) v[e] *= inv;
+            pg_store4(out + q * D + c, v);
+        }
+    };
+    for (int x = tid; x < g * D4; x += 32 * PD_WARPS) {
+        const int q = x / D4, c = x % D4 * 4;
+        float my[PD_WARPS], mx = -INFINITY, lv = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int y = 0; y < PD_WARPS; ++y) { my[y] = sm[y * g + q]; mx = fmaxf(mx, my[y]); }
 #pragma unroll
         for (int y = 0; y < PD_WARPS; ++y) {
-            const float c = sm[y * g + q] == -INFINITY ? 0.0f : pg_exp2(sm[y * g + q] - mx);
-            ov += c * so[y * g * D + x];
-            lv += c * ss[y * g + q];
+            const float f = my[y] == -INFINITY ? 0.0f : pg_exp2(my[y] - mx);
+            const float4 u = *(const float4 *) (so + (y * g + q) * D + c);
+            v[0] = fmaf(f, u.x, v[0]); v[1] = fmaf(f, u.y, v[1]); v[2] = fmaf(f, u.z, v[2]); v[3] = fmaf(f, u.w, v[3]);
+            lv += f * ss[y * g + q];
         }
-        co[x] = ov;
-        if (x % D == 0) { cm[q] = mx; cl[q] = lv; }
-    }
-    if (nrank > 1) pg_cluster_sync(); else __syncthreads();
-    // join the cluster's CTAs, each an equal share of the outputs
-    QT * out = (QT *) a.out + (long long) i * a.out_stride + h * g * D;
-    for (int x = rank * 32 * PD_WARPS + tid; x < g * D; x += nrank * 32 * PD_WARPS) {
-        const int q = x / D;
-        float mx = -INFINITY, ov = 0.0f, lv = 0.0f;
-        for (int y = 0; y < nrank; ++y) {
-            const float my = pg_dsm(cm + q, y), oy = pg_dsm(co + x, y), ly = pg_dsm(cl + q, y);
-            const float mn = fmaxf(mx, my);
-            const float c = mx == -INFINITY ? 0.0f : pg_exp2(mx - mn), d = my == -INFINITY ? 0.0f : pg_exp2(my - mn);
-            ov = ov * c + oy * d; lv = lv * c + ly * d;
-            mx = mn;
-        }
-        if (a.part && px >= 0) {                   // the tile kernel adds the prefix's part
-            float * rec = a.part + ((long long) i * a.n_head + h * g + q) * (D + 4);
-            rec[x % D] = ov;
-            if (x % D == 0) { rec[D] = mx; rec[D + 1] = lv; }
+        if (nrank == 1) {
+            finish(q, c, mx, lv, v);
         } else {
-            out[x] = pg_from<QT>(lv == 0.0f ? 0.0f : ov / lv);
+            pg_store4(co + q * D + c, v);
+            if (c == 0) { cm[q] = mx; cl[q] = lv; }
         }
     }
-    if (nrank > 1) pg_cluster_sync();              // no CTA leaves while another reads its shared memory
+    if (nrank == 1) return;
+    pg_cluster_sync();
+    for (int x = rank * 32 * PD_WARPS + tid; x < g * D4; x += nrank * 32 * PD_WARPS) {
+        const int q = x / D4, c = x % D4 * 4;
+        float my[8], ly[8], u[8][4], mx = -INFINITY, lv = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {              // every CTA's in flight at once
+            const int yy = min(y, nrank - 1);
+            my[y] = y < nrank ? pg_dsm(cm + q, yy) : -INFINITY; ly[y] = pg_dsm(cl + q, yy);
+            pg_dsm4(u[y], co + q * D + c, yy);
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) mx = fmaxf(mx, my[y]);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            const float f = my[y] == -INFINITY ? 0.0f : pg_exp2(my[y] - mx);
+            lv += f * ly[y];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(f, u[y][e], v[e]);
+        }
+        finish(q, c, mx, lv, v);
+    }
+    pg_cluster_sync();                             // no CTA leaves while another reads its shared memory
 }
 
 // ---- many rows: tcgen05 tiles ------------------------------------------------
@@ -1583,10 +1640,12 @@ cudaError_t pg_launch_tiles_nt(const t3b_shared_attn & a, const PgAttn & p, cuda
     // each request (prefix) may end in a part-filled tile
     const int64_t parts = PARTIAL ? p.n_prefix : p.n, rows = PARTIAL ? p.n : p.rows;
     const int64_t tiles = std::min((rows * p.group + ROWS - 1) / ROWS + parts - 1, rows * p.group);
+    // as many as there are if the rows are spread evenly: the others' CTAs leave at once
+    const int64_t even = std::min(tiles, parts * ((rows * p.group + parts * ROWS - 1) / (parts * ROWS)));
     const int64_t keys = ((PARTIAL ? 0 : (int64_t) a.max_blocks) + (a.n_prefix > 0 ? a.prefix_max_blocks : 0)) * a.cache.page_size;
     if (tiles * p.n_kv_head > (1 << 27)) return cudaErrorInvalidConfiguration;
     int c = 1;
-    while (c < 8 && tiles * p.n_kv_head * 2 * c <= (c < 4 ? 148 : 64) && ((PARTIAL && c < 4) || keys > (int64_t) 2 * PT_BN * c)) c *= 2;
+    while (c < 8 && even * p.n_kv_head * 2 * c <= (c < 4 ? 148 : 64) && ((PARTIAL && c < 4) || keys > (int64_t) 2 * PT_BN * c)) c *= 2;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
