@@ -1613,7 +1613,7 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(c, (unsigned) p.n_kv_head, (unsigned) p.n); cfg.blockDim = dim3(32 * PD_WARPS);
-    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = 1;
+    cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = c > 1;
     return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
 }
 
