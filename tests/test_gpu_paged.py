@@ -210,7 +210,7 @@ def test_captured_plan_evolves_its_state(pkg):
 
 @pytest.mark.parametrize("src,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("rows,kv,dim,page,pad,gap", [(1, 1, 64, 8, 0, 0), (5, 16, 64, 16, 0, 0), (333, 3, 128, 32, 24, 8),
-                                                      (2049, 8, 128, 64, 0, 8 * 64 * 128), (64, 2, 64, 256, 8, 0)])
+                                                      (2049, 8, 128, 64, 0, 8 * 64 * 128), (64, 2, 64, 256, 8, 0), (9001, 8, 64, 16, 16, 0)])
 def test_append_matches_its_definition(pkg, src, cache, rows, kv, dim, page, pad, gap):
     t = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
     ids = {"f32": 0, "f16": 1, "bf16": 30}
