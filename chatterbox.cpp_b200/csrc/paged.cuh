@@ -1224,6 +1224,7 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
         // o_full means that every MMA of the CTA has read them
         asm volatile("bar.sync 1, %0;" ::"n"(ROWS) : "memory");
         if (x < nt) {
+            float big = 0.0f;                      // not finite if an element is not
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 unsigned u[32];
@@ -1239,16 +1240,18 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
 #pragma unroll
                     for (int e = 0; e < 32; ++e) u[e] = 0u;
                 }
+                if (!PARTIAL)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) big += fabsf(__uint_as_float(u[e])) * 0x1p-16f;   // (32-bit sums of 16-bit V stay in range)
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
                     *(uint4 *) (so + r * (D + 4) + c + e) = make_uint4(u[e], u[e + 1], u[e + 2], u[e + 3]);
             }
-            s_m[r] = m; s_l[r] = l;
+            s_m[r] = m; s_l[r] = big < INFINITY ? l : NAN;            // NaN: the row is worked out again at the end
             const long long qrow = t.row0 + tok;
             const int head = h * g + row % g;
             s_off[r] = qrow * a.out_stride + (long long) head * D;
             if (PARTIAL) s_rec[r] = (qrow * a.n_head + head) * (D + 4);
-            s_odd[r] = 0;
         }
         if (NT == 1) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
     } else {
@@ -1457,16 +1460,17 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
         const float inv = lv == 0.0f ? 0.0f : 1.0f / lv;
 #pragma unroll
         for (int y = 0; y < 8; ++y) if (y < nrank) s_w[y * ROWS + tid] = my[y] * inv;
+        if (!PARTIAL) s_odd[tid] = !(lv < INFINITY);
         if (PARTIAL) s_wo[tid] = lo < 0.0f ? -1.0f : wo * inv;        // -1: the request is refused
     }
-    __syncthreads();
+    const bool odd = __syncthreads_or(!PARTIAL && tid < r_end - r_beg && s_odd[tid]);
     constexpr int C4 = D / 4;
-    bool odd = false;                              // a value that is not finite
     auto pieces = [&](auto ranks) {                // the parts' number at compile time: their loads in flight at once
         constexpr int N = decltype(ranks)::value;
 #pragma unroll(N <= 2 ? 4 : 1)
         for (int x = tid; x < (r_end - r_beg) * C4; x += THREADS) {
             const int rr = x / C4, r = r_beg + rr, c = x % C4 * 4;
+            if (!PARTIAL && s_odd[rr]) continue;   // (q may be out: the row's q is still needed)
             float v[4], u[N][4];
             float4 own;
             if (PARTIAL) own = __ldcg((const float4 *) (a.part + s_rec[r] + c));
@@ -1491,10 +1495,6 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
                 if (w != -1.0f) pg_store4((QT *) a.out + s_off[r] + c, v);
             } else {
                 pg_store4((QT *) a.out + s_off[r] + c, v);
-                if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
-                    s_odd[rr] = 1;
-                    odd = true;
-                }
             }
         }
     };
@@ -1502,7 +1502,7 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     else if (nrank == 2) pieces(std::integral_constant<int, 2>{});
     else if (nrank == 4) pieces(std::integral_constant<int, 4>{});
     else pieces(std::integral_constant<int, 8>{});
-    if (!PARTIAL && __syncthreads_or(odd))         // those rows again, by their keys one by one
+    if (!PARTIAL && odd)                           // rows that are not finite again, by their keys one by one
         for (int rr = warp; rr < r_end - r_beg; rr += THREADS / 32) {
             if (!s_odd[rr]) continue;
             const int row = t.lo + r_beg + rr, tok = row / g;
@@ -1553,7 +1553,7 @@ const char * pg_attn_wrong(const t3b_shared_attn & a, bool prompt, bool pointers
         return "q's type is neither the cache's nor T3B_F32 over an F16 cache";
     if (a.n_head <= 0 || a.n_head % a.cache.n_kv_head || a.n_head / a.cache.n_kv_head > 16)
         return "n_head is not 1 to 16 times n_kv_head";
-    if (a.n <= 0 || a.n > 65535 || a.n_prefix < 0 || a.n_prefix > 65535 || a.rows < 0) return "n, n_prefix or rows is out of range";
+    if (a.n <= 0 || a.n > 65535 || a.n_prefix < 0 || a.n_prefix > 65535 || a.rows < 0 || a.rows > 1 << 26) return "n, n_prefix or rows is out of range";
     if (a.max_blocks <= 0 || (int64_t) a.max_blocks * a.cache.page_size > 0x3fffffffll ||
         (a.n_prefix > 0 && (a.prefix_max_blocks <= 0 || (int64_t) a.prefix_max_blocks * a.cache.page_size > 0x3fffffffll)))
         return "max_blocks or prefix_max_blocks is out of range";

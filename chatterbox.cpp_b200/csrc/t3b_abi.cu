@@ -1773,9 +1773,10 @@ extern "C" int t3b_op_check(void * cuda_stream) {
         w |= v;
     }
     if (w) {
-        set_err(nullptr, "op-level device check failed (error word 0x%x:%s%s%s%s)", w,
+        set_err(nullptr, "op-level device check failed (error word 0x%x:%s%s%s%s%s)", w,
                 (w & T3B_DEVERR_POS) ? " length-out-of-range" : "", (w & T3B_DEVERR_TOKEN) ? " token-out-of-range" : "",
-                (w & T3B_DEVERR_PAGE) ? " page-out-of-range" : "", (w & T3B_DEVERR_FULL) ? " out-of-pages-or-rows" : "");
+                (w & T3B_DEVERR_PAGE) ? " page-out-of-range" : "", (w & T3B_DEVERR_FULL) ? " out-of-pages-or-rows" : "",
+                (w & T3B_DEVERR_TIMEOUT) ? " wait-ran-out" : "");
         return T3B_ERR_DEVICE;
     }
     return T3B_OK;

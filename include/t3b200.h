@@ -437,7 +437,7 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  *   AFTER the append.  rows bounds row_start[n]; rows of out from
  *   row_start[n] on stay as they were.
  *
- * A row with no key at all is zero.  A request whose length is negative or
+ * A row with no key at all (or only scores of -infinity) is zero.  A request whose length is negative or
  * past its table, or whose rows exceed its length, and a prefix length past
  * its table leave their rows unwritten and are reported; a page id outside
  * the pool is reported and its keys count as absent.
@@ -450,7 +450,7 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  * and their strides are multiples of 16 bytes.  out may be q (with the same
  * stride).  workspace holds t3b_op_attention_shared_workspace() bytes, 16-byte
  * aligned; calls that can run at the same time need one each.  n and
- * n_prefix <= 65535. */
+ * n_prefix <= 65535, rows <= 2^26. */
 typedef struct t3b_shared_attn {
     t3b_paged_kv    cache;
     const void *    q;

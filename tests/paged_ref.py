@@ -46,7 +46,7 @@ class Batch:
     ids outside the pool, so that a read of either shows."""
 
     def __init__(self, kind, lens, heads, kv_heads, dim, page, prefix_lens=(), prefix_start=None, adds=None, seed=0,
-                 gap=0, q_scale=1.0, q_pad=0, spare=3, pages_at=0, device="cuda"):
+                 gap=0, q_scale=1.0, q_pad=0, spare=3, pages_at=0, device="cuda", share=False):
         g = torch.Generator().manual_seed(seed)
         qt, ct, self.q_id, self.c_id = TYPES[kind]
         self.kind, self.heads, self.kv, self.dim, self.page = kind, heads, kv_heads, dim, page
@@ -55,6 +55,10 @@ class Batch:
         self.prefix_start = list(prefix_start) if prefix_start is not None else [0] + [n] * len(self.prefix_lens)
         width = max(1, max(blocks(max(x, 0), page) for x in lens)) + 1
         pwidth = max([1] + [blocks(x, page) for x in self.prefix_lens]) + 1
+        if share and len(self.prefix_lens) < n:
+            # a decode call computes a prefix once for the batch where re-reading it could cost over 48 MB,
+            # judged by the room in the prefix table: leave that much room
+            pwidth = max(pwidth, blocks(50e6 / (4 * kv_heads * dim * (n - max(1, len(self.prefix_lens)))) + page, page))
         used = sum(blocks(max(x, 0), page) for x in lens) + sum(blocks(x, page) for x in self.prefix_lens)
         self.n_pages = pages_at + used + spare
         ids = (pages_at + torch.randperm(used + spare, generator=g)).tolist()

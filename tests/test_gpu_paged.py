@@ -290,12 +290,14 @@ LAYOUTS = [(1, 1, 64, 16), (4, 4, 64, 8), (16, 16, 64, 16), (8, 2, 128, 32), (6,
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("share", [False, True])
 @pytest.mark.parametrize("heads,kv,dim,page", LAYOUTS)
-def test_decode_attention_matches_fp64(pkg, kind, heads, kv, dim, page):
+def test_decode_attention_matches_fp64(pkg, kind, heads, kv, dim, page, share):
     lens = [1, 0, page - 1, page, page + 1, 2 * page + 3, 63, 64, 65, 300, 129]
     for prefix, start in (([], None), ([1], [0, 11]), ([page + 3, 0, 200], [1, 4, 6, 10]), ([64, 128], [0, 1, 11])):
-        b = Batch(kind, lens, heads, kv, dim, page, prefix, start, seed=heads * 7 + len(prefix), gap=8 * len(prefix), q_pad=8 * len(prefix))
-        _attend(pkg, b)
+        b = Batch(kind, lens, heads, kv, dim, page, prefix, start, seed=heads * 7 + len(prefix), gap=8 * len(prefix), q_pad=8 * len(prefix), share=share)
+        d = _attend(pkg, b)
+        assert (d.workspace_bytes > 0) == (share and len(prefix) > 0)
         _close(b)
 
 
@@ -305,9 +307,10 @@ def test_decode_attention_matches_fp64(pkg, kind, heads, kv, dim, page):
     (130, 4, 2, 64, 16, 77, 1, 40), (65, 32, 8, 128, 32, 1000, 1, 90), (300, 2, 1, 64, 8, 513, 0, 30), (1, 1, 1, 128, 16, 4000, 0, 1)])
 def test_decode_attention_sizes(pkg, kind, n, heads, kv, dim, page, prefix, lo, hi):
     rng = np.random.default_rng(n + heads)
-    b = Batch(kind, rng.integers(lo, hi + 1, n).tolist(), heads, kv, dim, page, [prefix], [0, n], seed=n)
-    _attend(pkg, b)
-    _close(b)
+    for share in (False, True):
+        b = Batch(kind, rng.integers(lo, hi + 1, n).tolist(), heads, kv, dim, page, [prefix], [0, n], seed=n, share=share)
+        _attend(pkg, b)
+        _close(b)
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
@@ -331,12 +334,13 @@ def test_prompt_attention_sizes(pkg, kind, adds, past, heads, kv, dim, page, pre
     _close(b)
 
 
-@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
 @pytest.mark.parametrize("kind,q_scale", [("f32", 3e4), ("f32", 1e-6), ("f16", 100.0), ("bf16", 300.0), ("f32", 0.0)])
-def test_large_and_small_queries(pkg, kind, q_scale, prompt):
+def test_large_and_small_queries(pkg, kind, q_scale, prompt, share):
     """Scores of thousands (the softmax picks one key) and of nothing (it averages)."""
     lens = [40, 200, 1]
-    b = Batch(kind, lens, 4, 2, 64, 16, [100], [0, 3], adds=[40, 30, 1] if prompt else None, seed=3, q_scale=q_scale)
+    b = Batch(kind, lens, 4, 2, 64, 16, [100], [0, 3], adds=[40, 30, 1] if prompt else None, seed=3, q_scale=q_scale,
+              share=share)
     _attend(pkg, b)
     ref, tol = b.reference()
     got = b.out_all[:b.rows].cpu().double()
@@ -344,10 +348,11 @@ def test_large_and_small_queries(pkg, kind, q_scale, prompt):
     assert ((got - ref).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
 @pytest.mark.parametrize("scale", [0.3, -0.125])
-def test_scale_argument(pkg, prompt, scale):
-    b = Batch("f32", [40, 100], 4, 2, 64, 16, [50], [0, 2], adds=[40, 30] if prompt else None, seed=4)
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+def test_scale_argument(pkg, prompt, share, scale, kind):
+    b = Batch(kind, [40, 100], 4, 2, 64, 16, [50], [0, 2], adds=[40, 30] if prompt else None, seed=4, share=share)
     d = b.desc(pkg)
     d.scale = scale
     f = pkg.lib().t3b_op_attention_shared_prompt if prompt else pkg.lib().t3b_op_attention_shared
@@ -356,11 +361,15 @@ def test_scale_argument(pkg, prompt, scale):
     _close(b, scale=scale)
 
 
-@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("kind,prefix", [("f32", 70), ("f16", 70), ("bf16", 70), ("f32", 2000), ("bf16", 2000)])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
-def test_non_finite_values_of_later_tokens_stay_there(pkg, kind, value):
-    """A NaN or infinity in the K or V of a token reaches the rows that see it, and no row before it."""
-    b = Batch(kind, [100, 30], 6, 2, 64, 16, [70], [0, 2], adds=[60, 30], seed=31)
+def test_non_finite_values_of_later_tokens_stay_there(pkg, kind, prefix, value, in_place):
+    """A NaN or infinity in the K or V of a token reaches the rows that see
+    it, and no row before it; also where out is q, and where the keys are
+    split over CTAs (the long prefix)."""
+    b = Batch(kind, [100, 30], 6, 2, 64, 16, [prefix], [0, 2], adds=[60, 30], seed=31)
+    q = b.q_all.clone()
     ref, tol = b.reference()
     key = 85                                                      # own key 85 of request 0: rows from 45 on see it
     slot = int(b.table[0, key // 16]), key % 16
@@ -369,9 +378,10 @@ def test_non_finite_values_of_later_tokens_stay_there(pkg, kind, value):
         old = view[slot[0], 1, slot[1]].clone()
         view[slot[0], 1, slot[1], dims] = value                   # kv head 1: query heads 3, 4 and 5
         b.out_all.fill_(-7)
-        _attend(pkg, b)
+        _attend(pkg, b, out=b.q_all if in_place else None)
         view[slot[0], 1, slot[1]] = old
-        got = b.out_all[:90].cpu().double()
+        got = (b.q_all if in_place else b.out_all)[:90].cpu().double()
+        b.q_all.copy_(q)
         clean = torch.ones_like(ref, dtype=torch.bool)
         clean[45:60, 3 * 64:] = False
         assert ((got - ref).abs() <= tol)[clean].all()
@@ -382,10 +392,10 @@ def test_non_finite_values_of_later_tokens_stay_there(pkg, kind, value):
                 assert torch.isnan(hit).all()
 
 
-@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
-def test_output_in_place_of_q(pkg, prompt, kind):
-    b = Batch(kind, [40, 3, 700], 8, 4, 64, 16, [300], [0, 3], adds=[40, 2, 300] if prompt else None, seed=5)
+def test_output_in_place_of_q(pkg, prompt, share, kind):
+    b = Batch(kind, [40, 3, 700], 8, 4, 64, 16, [300], [0, 2], adds=[40, 2, 300] if prompt else None, seed=5, share=share)
     out = b.q_all.clone()
     b.q_all, b.q = out, out[:, :8 * 64]
     ref, tol = b.reference()
@@ -393,20 +403,22 @@ def test_output_in_place_of_q(pkg, prompt, kind):
     assert ((out.cpu().double() - ref).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("prompt", [False, True])
-def test_bad_lengths_and_pages_are_reported(pkg, prompt):
+@pytest.mark.parametrize("prompt,shared", [(False, False), (False, True), (True, False)])
+def test_bad_lengths_and_pages_are_reported(pkg, prompt, shared):
     """A request with a bad length leaves its rows unwritten, a bad page's
-    keys count as absent, and the other requests are right."""
+    keys count as absent, and the other requests are right; also where the
+    prefix is computed once for the batch (long enough for that)."""
     lens, adds = [40, 30, 20, 50], [3, 30, 2, 1]
     for what in ("long", "negative", "page", "prefix"):
-        b = Batch("f32", lens, 4, 2, 64, 16, [20, 20], [0, 2, 4], adds=adds if prompt else None, seed=6)
+        b = Batch("f32", lens, 4, 2, 64, 16, [20, 20], [0, 2, 4], adds=adds if prompt else None, seed=6, share=shared)
         skip = [1]
+        assert (b.desc(pkg).workspace_bytes > 0) == shared
         if what == "long":
             b.len[1] = b.table.shape[1] * 16 + 1
         elif what == "negative":
             b.len[1] = -3
         elif what == "prefix":
-            b.plen[0], skip = 100, [0, 1]
+            b.plen[0], skip = 16 * b.ptable.shape[1] + 1, [0, 1]
         else:
             b.table[1, 0] = [b.n_pages, -1][prompt]
         _attend(pkg, b)
@@ -433,9 +445,10 @@ def test_more_rows_than_keys_are_reported(pkg):
 
 def test_a_workspace_of_another_call_leaves_no_trace(pkg):
     """Two batches through one workspace, one after the other and back."""
-    x = Batch("f32", [40] * 20, 4, 4, 64, 16, [300], [0, 20], seed=7)
-    y = Batch("f32", [3, 500], 4, 4, 64, 16, [20, 700], [0, 1, 2], seed=8)
+    x = Batch("f32", [40] * 20, 4, 4, 64, 16, [300], [0, 20], seed=7, share=True)
+    y = Batch("f32", [3, 500, 60], 4, 4, 64, 16, [20, 700], [0, 1, 3], seed=8, share=True)
     dx, dy = x.desc(pkg), y.desc(pkg)
+    assert dx.workspace_bytes > 0 and dy.workspace_bytes > 0
     big = torch.empty(max(dx.workspace_bytes, dy.workspace_bytes, 16), dtype=torch.uint8, device="cuda").fill_(0xFF)
     for b, d in ((x, dx), (y, dy), (x, dx)):
         d.workspace, d.workspace_bytes = big.data_ptr(), big.numel()
@@ -445,9 +458,9 @@ def test_a_workspace_of_another_call_leaves_no_trace(pkg):
         _close(b)
 
 
-@pytest.mark.parametrize("prompt", [False, True])
-def test_repeated_calls_give_the_same_bits(pkg, prompt):
-    b = Batch("f32", [40, 900, 7, 333], 8, 8, 64, 16, [377], [0, 4], adds=[40, 60, 7, 100] if prompt else None, seed=9)
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
+def test_repeated_calls_give_the_same_bits(pkg, prompt, share):
+    b = Batch("f32", [40, 900, 7, 333], 8, 8, 64, 16, [377], [0, 4], adds=[40, 60, 7, 100] if prompt else None, seed=9, share=share)
     _attend(pkg, b)
     first = b.out_all.clone()
     for _ in range(5):
@@ -455,25 +468,28 @@ def test_repeated_calls_give_the_same_bits(pkg, prompt):
         assert torch.equal(b.out_all, first)
 
 
-def test_two_calls_at_once_on_two_streams(pkg):
-    bs = [Batch("f32", [200, 30, 77] * 8, 8, 8, 64, 16, [377], [0, 24], seed=10 + i) for i in range(2)]
+@pytest.mark.parametrize("kind", ["prompt", "decode", "shared"])
+def test_two_calls_at_once_on_two_streams(pkg, kind):
+    bs = [Batch("f32", [200, 30, 77] * 8, 8, 8, 64, 16, [377], [0, 24], adds=[150, 30, 1] * 8 if kind == "prompt" else None,
+                seed=10 + i, share=kind == "shared") for i in range(2)]
     ds = [b.desc(pkg) for b in bs]
+    f = pkg.lib().t3b_op_attention_shared_prompt if kind == "prompt" else pkg.lib().t3b_op_attention_shared
     streams = [torch.cuda.Stream() for _ in range(2)]
     torch.cuda.synchronize()
     for _ in range(20):
         for d, s in zip(ds, streams):
-            pkg.check(pkg.lib().t3b_op_attention_shared(C.byref(d), C.c_void_p(s.cuda_stream)))
+            pkg.check(f(C.byref(d), C.c_void_p(s.cuda_stream)))
     torch.cuda.synchronize()
     for b in bs:
         _close(b)
 
 
-@pytest.mark.parametrize("dim,prompt", [(64, False), (128, True)])
-def test_pages_past_2_to_the_31_elements(pkg, dim, prompt):
+@pytest.mark.parametrize("dim,prompt,share", [(64, False, False), (128, False, True), (128, True, False)])
+def test_pages_past_2_to_the_31_elements(pkg, dim, prompt, share):
     """Page offsets that do not fit 32 bits: K and V of 4.4 GB each."""
     page, kv = 64, 8
     at = (1 << 31) // (page * kv * dim) + 3
-    b = Batch("f16", [70, 200], 8, kv, dim, page, [100], [0, 2], adds=[70, 10] if prompt else None, seed=11, pages_at=at)
+    b = Batch("f16", [70, 200], 8, kv, dim, page, [300], [0, 2], adds=[70, 10] if prompt else None, seed=11, pages_at=at, share=share)
     assert b.k.numel() > 1 << 31
     _attend(pkg, b)
     _close(b)
@@ -483,8 +499,9 @@ def test_pages_past_2_to_the_31_elements(pkg, dim, prompt):
 # the operators together
 # --------------------------------------------------------------------------
 
+@pytest.mark.parametrize("share", [False, True])
 @pytest.mark.parametrize("graph", [False, True])
-def test_a_serving_loop_matches_dense_attention(pkg, graph):
+def test_a_serving_loop_matches_dense_attention(pkg, graph, share):
     """Plan, append and attention as a server runs them: prompts of a common
     prefix are admitted, decode, finish, and their slots are taken over by
     others; every step's output equals t3b_op_attention on dense caches that
@@ -499,7 +516,9 @@ def test_a_serving_loop_matches_dense_attention(pkg, graph):
     pre_pages = blocks(P, page)
     dense = torch.zeros(2, n, H, 256, D, dtype=torch.float16, device="cuda")
     kvp = torch.randn(2, P, H, D, generator=g, device="cuda").half()
-    ptable = torch.arange(pre_pages, dtype=torch.int32, device="cuda")
+    room = 200 if share else pre_pages                   # 3200 keys of room: the prefix is computed once for the batch
+    ptable = torch.full((room,), -1, dtype=torch.int32, device="cuda")
+    ptable[:pre_pages] = torch.arange(pre_pages)
     for t in range(P):
         pool[:, t // page, :, t % page] = kvp[:, t]
     dense[:, :, :, :P] = kvp.permute(0, 2, 1, 3)[:, None]
@@ -518,9 +537,10 @@ def test_a_serving_loop_matches_dense_attention(pkg, graph):
     dapp = pkg.KvAppend(cache=cache, k=p(k), v=p(v), stride=H * D, slots=p(slots), dtype=0, rows=cap)
     da = pkg.SharedAttn(cache=cache, q=p(q), out=p(out), q_stride=H * D, out_stride=H * D, len=p(ln), table=p(table),
                         row_start=p(row_start), prefix_start=p(pstart), prefix_len=p(plen), prefix_table=p(ptable), dtype=0,
-                        n_head=H, n=n, rows=cap, max_blocks=width, n_prefix=1, prefix_max_blocks=pre_pages)
+                        n_head=H, n=n, rows=cap, max_blocks=width, n_prefix=1, prefix_max_blocks=room)
     dd = pkg.SharedAttn.from_buffer_copy(da)
     dd.rows, dd.row_start = n, None
+    assert (L.t3b_op_attention_shared_workspace(C.byref(dd)) > 0) == share
     size = max(L.t3b_op_attention_shared_workspace(C.byref(da)), L.t3b_op_attention_shared_workspace(C.byref(dd)))
     ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
     for d in (da, dd):

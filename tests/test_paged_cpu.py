@@ -49,7 +49,7 @@ def test_bad_caches_are_refused(pkg, cache):
                                  dict(n_prefix=70000), dict(max_blocks=0), dict(max_blocks=1 << 27),
                                  dict(prefix_max_blocks=0), dict(prefix_max_blocks=1 << 27), dict(q_stride=511),
                                  dict(q_stride=508), dict(out_stride=514), dict(out_stride=0), dict(scale=float("nan")),
-                                 dict(scale=float("inf")), dict(rows=-1), dict(q_stride=516)], ids=str)
+                                 dict(scale=float("inf")), dict(rows=-1), dict(rows=(1 << 26) + 1), dict(q_stride=516)], ids=str)
 def test_bad_attention_calls_are_refused(pkg, bad):
     L = pkg.lib()
     for f in (L.t3b_op_attention_shared, L.t3b_op_attention_shared_prompt):
