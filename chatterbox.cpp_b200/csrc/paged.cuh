@@ -56,15 +56,15 @@ __device__ __forceinline__ int pg_find(const int * at, int n, int x) {
     return lo;
 }
 
-// Rows r0 .. r0 + 3 of the row maps: one bisection of s_row (n + 1 first
-// rows) and, mostly, one page id for all four.  start(i): the own tokens
+// Rows r0 .. r0 + E - 1 of the row maps: one bisection of s_row (n + 1 first
+// rows) and, mostly, one page id for all of them.  start(i): the own tokens
 // before the step; page(i, b): table entry b of request i.
-template <class Start, class Page>
+template <int E, class Start, class Page>
 __device__ __forceinline__ void pg_plan_rows(const t3b_kv_plan & p, int n, int nrow, int lg, int r0, const int * s_row, Start start, Page page) {
-    int req[4], pos[4], slot[4];
+    int req[E], pos[E], slot[E];
     int i = r0 < nrow ? pg_find(s_row, n, r0) : 0, have = -1, id = -1, ln = r0 < nrow ? start(i) : 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < E; ++e) {
         const int r = r0 + e;
         req[e] = pos[e] = slot[e] = -1;
         if (r >= nrow) continue;
@@ -86,13 +86,13 @@ __device__ __forceinline__ void pg_plan_rows(const t3b_kv_plan & p, int n, int n
         }
         if (id >= 0) slot[e] = (id << lg) + (pos[e] & ((1 << lg) - 1));
     }
-    if (((((uintptr_t) p.row_req) | ((uintptr_t) p.row_pos) | ((uintptr_t) p.slots)) & 15) == 0 && r0 + 4 <= p.rows_cap) {
-        if (p.row_req) *(int4 *) (p.row_req + r0) = make_int4(req[0], req[1], req[2], req[3]);
-        if (p.row_pos) *(int4 *) (p.row_pos + r0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-        if (p.slots) *(int4 *) (p.slots + r0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    if (((((uintptr_t) p.row_req) | ((uintptr_t) p.row_pos) | ((uintptr_t) p.slots)) & 15) == 0 && E == 4 && r0 + 4 <= p.rows_cap) {
+        if (p.row_req) *(int4 *) (p.row_req + r0) = make_int4(req[0], req[E / 4], req[E / 2], req[E - 1]);
+        if (p.row_pos) *(int4 *) (p.row_pos + r0) = make_int4(pos[0], pos[E / 4], pos[E / 2], pos[E - 1]);
+        if (p.slots) *(int4 *) (p.slots + r0) = make_int4(slot[0], slot[E / 4], slot[E / 2], slot[E - 1]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < E; ++e) {
             if (r0 + e >= p.rows_cap) break;
             if (p.row_req) p.row_req[r0 + e] = req[e];
             if (p.row_pos) p.row_pos[r0 + e] = pos[e];
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(t3b_kv_plan p) {
     if (r0 >= p.rows_cap) return;
     auto start = [&](int i) { return p.len_out ? __ldcg(p.len_out + i) - (pg_sm[i + 1] - pg_sm[i]) : __ldcg(p.len + i); };
     auto page = [&](int i, int blk) { return __ldcg(p.table + (size_t) i * p.max_blocks + blk); };
-    pg_plan_rows(p, n, pg_sm[n], lg, r0, pg_sm, start, page);
+    pg_plan_rows<4>(p, n, pg_sm[n], lg, r0, pg_sm, start, page);
 }
 
 // One cluster.  Every CTA scans all requests (a few KB), so all of them know
@@ -193,7 +193,11 @@ __global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p, bo
             return blk < held ? p.table[(size_t) i * p.max_blocks + blk] : p.free_pages[top - 1 - (s_take[i] + blk - held)];
         };
         auto start = [&](int i) { return s_len[i]; };
-        for (int r0 = 4 * me; r0 < p.rows_cap; r0 += 4 * all) pg_plan_rows(p, n, nrow, lg, r0, s_row, start, page);
+        if (p.rows_cap <= all) {                   // a thread for each: the shortest way
+            if (me < p.rows_cap) pg_plan_rows<1>(p, n, nrow, lg, me, s_row, start, page);
+        } else {
+            for (int r0 = 4 * me; r0 < p.rows_cap; r0 += 4 * all) pg_plan_rows<4>(p, n, nrow, lg, r0, s_row, start, page);
+        }
     }
     for (int i = me; i < n; i += all) {
         p.row_start[i] = ok ? s_row[i] : 0;
@@ -1759,9 +1763,9 @@ int t3b_op_kv_plan(const t3b_kv_plan * p, void * cuda_stream) {
     }
     // one CTA does for few requests and rows; eight cost 0.3 us more and take a larger step's work apart
     const bool rows_here = p->rows_cap <= PG_PLAN_ROWS || (!p->row_req && !p->row_pos && !p->slots);
-    const int most = std::max(p->n, p->rows_cap / 4);
+    const int most = std::max(p->n, p->rows_cap);
     const unsigned threads = most <= 128 ? 128 : most <= 256 ? 256 : PG_PLAN_T;
-    const unsigned c = p->n <= PG_PLAN_T && p->rows_cap <= 4096 ? 1 : PG_PLAN_CLUSTER;
+    const unsigned c = p->n <= PG_PLAN_T && p->rows_cap <= PG_PLAN_T ? 1 : PG_PLAN_CLUSTER;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
