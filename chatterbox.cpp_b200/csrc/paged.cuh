@@ -451,10 +451,12 @@ __host__ __device__ constexpr int pd_stages(int D) { return D == 64 ? 3 : 2; }
 __host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D) * 2 * PD_TK * D * 2; }
 
 // grid = (splits, n_kv_head, n), clusters of `splits` CTAs, 128 threads
-template <class QT, class CT, int D, int MT>
+// MT: tiles of 16 rows; RH: their 8-row halves that hold queries of their own
+// (F32: one, the other has its lo parts; 16-bit: one up to 8 queries, then two)
+template <class QT, class CT, int D, int MT, int RH>
 __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAttn a) {
     constexpr bool F32 = sizeof(QT) == 4;
-    constexpr int RPM = F32 ? 8 : 16;              // queries of an M tile
+    constexpr int RPM = 8 * RH;                    // queries of an M tile
     constexpr int NS = pd_stages(D), KS = D / 16, CH = D / 8;
     constexpr int TILE = PD_TK * D * 2;            // bytes of a K or a V tile
     constexpr float BIAS = PgBias<CT>::v;
@@ -488,7 +490,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int r = mt * RPM + (lane >> 2) + (b & 1) * 8;
-                    qf[mt][k][b] = r < g ? *(const unsigned *) ((const CT *) a.q + (long long) i * a.q_stride + (h * g + r) * D +
+                    qf[mt][k][b] = (b & 1) < RH && r < g ? *(const unsigned *) ((const CT *) a.q + (long long) i * a.q_stride + (h * g + r) * D +
                                                                 k * 16 + (b >> 1) * 8 + (lane & 3) * 2)
                                          : 0u;
                 }
@@ -595,7 +597,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 #pragma unroll
     for (int x = 0; x < NS - 1; ++x) issue(x, ids, x);
 
-    float sc[MT][2];                               // what a score of row lane / 4 (+ 8) is multiplied by
+    float sc[MT];                                  // what a score is multiplied by
     const float sl2 = a.scale * 1.4426950408889634f;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -614,21 +616,22 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const int e = pg_row_exp(mx);
             const float f = pg_pow2(-e);
-            sc[mt][0] = sc[mt][1] = pg_pow2(e);
+            sc[mt] = pg_pow2(e);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int b = 0; b < 2; ++b) pg_split2(qv[mt][k][b].x * f, qv[mt][k][b].y * f, qf[mt][k][2 * b], qf[mt][k][2 * b + 1]);
         } else {
-            sc[mt][0] = sc[mt][1] = sl2;
+            sc[mt] = sl2;
         }
     }
 
     float o[MT][D / 8][4];
-    float m[MT][2], l[MT][2];
+    float m[MT][RH], l[MT][RH];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        m[mt][0] = m[mt][1] = -INFINITY; l[mt][0] = l[mt][1] = 0.0f;
+#pragma unroll
+        for (int r = 0; r < RH; ++r) { m[mt][r] = -INFINITY; l[mt][r] = 0.0f; }
 #pragma unroll
         for (int d = 0; d < D / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
     }
@@ -663,18 +666,22 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
         unsigned p[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            float z[2][4];                         // scores in units of log2, masked
+            float z[2][2 * RH];                    // scores in units of log2: two keys for each half's row, twice
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float raw = F32 ? s[mt][nt][e & 1] + s[mt][nt][(e & 1) + 2] : s[mt][nt][e];
-                    z[nt][e] = (lane & 3) * 2 + (e & 1) < (nt ? n1 : n0) ? raw * sc[mt][e >> 1] : -INFINITY;
-                }
-            float top[2];
+                for (int e = 0; e < 2 * RH; ++e) z[nt][e] = (F32 ? s[mt][nt][e] + s[mt][nt][e + 2] : s[mt][nt][e]) * sc[mt];
+            if (n0 + n1 < PD_TK) {
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2 * RH; ++e)
+                        if ((lane & 3) * 2 + (e & 1) >= (nt ? n1 : n0)) z[nt][e] = -INFINITY;
+            }
+            float top[RH];
             bool grow = false;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RH; ++r) {
                 float t = fmaxf(fmaxf(z[0][2 * r], z[0][2 * r + 1]), fmaxf(z[1][2 * r], z[1][2 * r + 1]));
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
                 t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
@@ -683,15 +690,18 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             }
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int r = 0; r < RH; ++r) {
                     const float c = m[mt][r] == -INFINITY ? 0.0f : pg_exp2(m[mt][r] - top[r]);
                     m[mt][r] = top[r]; l[mt][r] *= c;
 #pragma unroll
-                    for (int d = 0; d < D / 8; ++d) { o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c; }
+                    for (int d = 0; d < D / 8; ++d) {
+                        o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c;
+                        if (F32) { o[mt][d][2] *= c; o[mt][d][3] *= c; }
+                    }
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int r = 0; r < RH; ++r) {
                 const float base = m[mt][r] == -INFINITY ? 0.0f : m[mt][r] - BIAS;
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
@@ -705,7 +715,10 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
                 pg_split2(z[1][0], z[1][1], p[mt][2], p[mt][3]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) p[mt][e] = pg_pack2<CT>(z[e >> 1][2 * (e & 1)], z[e >> 1][2 * (e & 1) + 1]);
+                for (int nt = 0; nt < 2; ++nt) {
+                    p[mt][2 * nt] = pg_pack2<CT>(z[nt][0], z[nt][1]);
+                    p[mt][2 * nt + 1] = RH == 2 ? pg_pack2<CT>(z[nt][2 * RH - 2], z[nt][2 * RH - 1]) : 0u;
+                }
             }
         }
 #pragma unroll
@@ -736,7 +749,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int r = 0; r < (F32 ? 1 : 2); ++r) {
+        for (int r = 0; r < RH; ++r) {
             const int q = mt * RPM + (lane >> 2) + r * 8;
             l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 1);
             l[mt][r] += __shfl_xor_sync(0xffffffffu, l[mt][r], 2);
@@ -1649,9 +1662,9 @@ template <class K> cudaError_t pg_allow_smem(K * kernel, int bytes) {
     return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-template <class QT, class CT, int D, int MT>
+template <class QT, class CT, int D, int MT, int RH>
 cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaStream_t st) {
-    const cudaError_t e = pg_allow_smem(attn_shared_decode_kernel<QT, CT, D, MT>, pd_smem(D));
+    const cudaError_t e = pg_allow_smem(attn_shared_decode_kernel<QT, CT, D, MT, RH>, pd_smem(D));
     if (e != cudaSuccess) return e;
     const unsigned c = (unsigned) pg_splits(a);
     cudaLaunchConfig_t cfg{};
@@ -1660,7 +1673,7 @@ cudaError_t pg_launch_decode(const t3b_shared_attn & a, const PgAttn & p, cudaSt
     at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(c, (unsigned) p.n_kv_head, (unsigned) p.n); cfg.blockDim = dim3(32 * PD_WARPS);
     cfg.dynamicSmemBytes = pd_smem(D); cfg.stream = st; cfg.attrs = at; cfg.numAttrs = c > 1;
-    return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT>, p);
+    return cudaLaunchKernelEx(&cfg, attn_shared_decode_kernel<QT, CT, D, MT, RH>, p);
 }
 
 // The pages of K or V as a 4-D tensor [n_pages][n_kv_head][page][D], boxes of
@@ -1721,9 +1734,10 @@ cudaError_t pg_launch_tiles(const t3b_shared_attn & a, const PgAttn & p, cudaStr
 template <class QT, class CT, int D>
 cudaError_t pg_launch_attention(const t3b_shared_attn & a, const PgAttn & p, bool prompt, cudaStream_t st) {
     if (!prompt) {
-        // F32 queries take two of an M tile's 16 rows
-        const cudaError_t e = sizeof(QT) == 4 && p.group > 8 ? pg_launch_decode<QT, CT, D, sizeof(QT) == 4 ? 2 : 1>(a, p, st)
-                                                             : pg_launch_decode<QT, CT, D, 1>(a, p, st);
+        // an M tile has 16 rows: 8 F32 queries, or 16 of 16 bits (the second half left out where it has none)
+        constexpr bool F32 = sizeof(QT) == 4;
+        const cudaError_t e = p.group > 8 ? pg_launch_decode<QT, CT, D, F32 ? 2 : 1, F32 ? 1 : 2>(a, p, st)
+                                          : pg_launch_decode<QT, CT, D, 1, 1>(a, p, st);
         return e != cudaSuccess || !p.part ? e : pg_launch_tiles<QT, CT, D, true>(a, p, st);
     }
     return pg_launch_tiles<QT, CT, D, false>(a, p, st);
