@@ -495,6 +495,93 @@ def test_pages_past_2_to_the_31_elements(pkg, dim, prompt, share):
     _close(b)
 
 
+@pytest.mark.parametrize("mode", ["decode", "shared", "prompt"])
+def test_more_than_32_prefixes(pkg, mode):
+    rng = np.random.default_rng(13)
+    start = np.cumsum(np.r_[1, rng.integers(0, 4, 41)]).tolist()   # some prefixes have no request, some requests no prefix
+    n = start[-1] + 2
+    adds = rng.integers(0, 9, n).tolist() if mode == "prompt" else None
+    lens = [int(x) + (a if adds else 0) for x, a in zip(rng.integers(0, 60, n), adds or [0] * n)]
+    b = Batch("f32", lens, 4, 2, 64, 16, rng.integers(0, 150, 41).tolist(), start, adds=adds, seed=14, share=mode == "shared")
+    _attend(pkg, b)
+    _close(b)
+
+
+@pytest.mark.parametrize("mode", ["decode", "prompt"])
+def test_as_many_requests_as_allowed(pkg, mode):
+    """65535 requests of one key each: every row is that key's V."""
+    n, page = 65535, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(n, 1, page, 64, generator=g, device="cuda").half()
+    v = torch.randn(n, 1, page, 64, generator=g, device="cuda").half()
+    q = torch.randn(n, 64, generator=g, device="cuda")
+    out = torch.full((n, 64), -7.0, device="cuda")
+    table, ln = torch.randperm(n, generator=g, device="cuda").to(torch.int32), torch.ones(n, dtype=torch.int32, device="cuda")
+    starts = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    d = pkg.SharedAttn(cache=pkg.PagedKv(k=k.data_ptr(), v=v.data_ptr(), dtype=1, n_pages=n, n_kv_head=1, page_size=page, head_dim=64),
+                       q=q.data_ptr(), out=out.data_ptr(), q_stride=64, out_stride=64, len=ln.data_ptr(), table=table.data_ptr(),
+                       row_start=starts.data_ptr(), dtype=0, n_head=1, n=n, rows=n, max_blocks=1)
+    f = pkg.lib().t3b_op_attention_shared if mode == "decode" else pkg.lib().t3b_op_attention_shared_prompt
+    pkg.check(f(C.byref(d), _stream()))
+    want = v[table.long(), 0, 0].float()
+    assert ((out - want).abs() <= want.abs() * 2.0 ** -20).all()      # one key: its weight is 1 to a few roundings
+
+
+def test_rows_without_a_request_stay_as_they_were(pkg):
+    """A prompt call whose requests bring no rows, with room for some."""
+    b = Batch("f32", [5, 0, 3], 4, 2, 64, 16, [20], [0, 3], adds=[0, 0, 0], seed=15)
+    b.q_all = torch.zeros(7, 256, device="cuda")
+    b.q = b.q_all
+    out = torch.full((7, 256), -7.0, device="cuda")
+    _attend(pkg, b, out=out, rows=7)
+    assert (out == -7).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_calls_one_after_the_other_without_waiting(pkg, kind):
+    """Two batches take turns on one stream through one workspace, nothing
+    waited for in between; what each left is copied right behind it."""
+    bs = [Batch(kind, lens, 8, 4, 64, 16, [p], [0, len(lens)], seed=16 + p, share=True)
+          for lens, p in (([40, 3, 200, 77] * 9, 700), ([5, 600], 90))]
+    ds = [b.desc(pkg) for b in bs]
+    big = torch.empty(max(d.workspace_bytes for d in ds), dtype=torch.uint8, device="cuda").fill_(0xFF)
+    left = []
+    for d in ds:
+        d.workspace, d.workspace_bytes = big.data_ptr(), big.numel()
+    for _ in range(25):
+        for b, d in zip(bs, ds):
+            b.out_all.fill_(-7)
+            pkg.check(pkg.lib().t3b_op_attention_shared(C.byref(d), _stream()))
+            left.append(b.out_all.clone())
+    torch.cuda.synchronize()
+    for b in bs:
+        _close(b)
+    assert all(torch.equal(x, left[i % 2]) for i, x in enumerate(left))
+
+
+def test_append_right_behind_a_large_plan(pkg):
+    """The row maps of a large step are there when the append that follows reads them."""
+    rng = np.random.default_rng(17)
+    n, page, width = 900, 16, 12
+    ln, add, release, table, free, n_free = _random_step(rng, n, page, width, True)
+    cap = int(add.sum()) + 100
+    ref = paged_ref.plan(ln, add, release, page, table, free, n_free, cap)
+    p = Plan(pkg, ln, add, release, page, table, free, n_free, cap, in_place=True)
+    assert cap > 16384
+    rows = torch.randn(2, cap, 64, device="cuda")
+    pool = torch.zeros(2, n * width, 1, page, 64, dtype=torch.float16, device="cuda")
+    a = pkg.KvAppend(cache=pkg.PagedKv(k=pool[0].data_ptr(), v=pool[1].data_ptr(), dtype=1, n_pages=n * width, n_kv_head=1, page_size=page,
+                                       head_dim=64),
+                     k=rows[0].data_ptr(), v=rows[1].data_ptr(), stride=64, slots=p.out["slots"].data_ptr(), dtype=0, rows=cap)
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    pkg.check(pkg.lib().t3b_op_kv_append(C.byref(a), _stream()))
+    torch.cuda.synchronize()
+    want = torch.zeros(2, n * width * page, 64, dtype=torch.float16)
+    live = torch.from_numpy(ref["slots"] >= 0)
+    want[:, torch.from_numpy(ref["slots"][ref["slots"] >= 0])] = rows.cpu()[:, live].half()
+    assert torch.equal(pool.cpu().view(2, -1, 64), want)
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
