@@ -19,7 +19,7 @@ static __device__ unsigned g_paged_err;
 #define PG_PLAN_CLUSTER 8
 #define PG_PLAN_ROWS 16384   // from this many rows on a kernel of its own fills them in
 
-// exclusive prefix sums of two 64-bit values over the CTA; `tot` gets the sums
+// exclusive prefix sums of two 64-bit values over the CTA; ta and tb get the sums
 __device__ __forceinline__ void pg_scan2(unsigned long long & a, unsigned long long & b, unsigned long long (*red)[2],
                                          unsigned long long & ta, unsigned long long & tb) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
@@ -102,8 +102,8 @@ __device__ __forceinline__ void pg_plan_rows(const t3b_kv_plan & p, int n, int n
 }
 
 // The row maps of a large step, over the whole GPU, from what the plan kernel
-// left: a step of 2048 requests and 200 000 rows took
-// 18 us in one cluster and takes 12 so.
+// left: a step of 2048 requests and 200 000 rows took 18 us in one cluster and
+// takes 12 so.
 __global__ __launch_bounds__(256) void kv_plan_rows_kernel(t3b_kv_plan p) {
     extern __shared__ int pg_sm[];
     const int n = p.n, lg = __ffs(p.page_size) - 1;
@@ -357,7 +357,10 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 // 128, prefix apart) run at 6.4 TB/s, 0.98 of the copy rate; 128 of 88 to
 // 1088 (f32, 16 x 64) at 5.6, where a quarter of a CTA's 12 us goes to its
 // first loads and its last join.  Two warps a CTA, deeper rings and a cluster
-// for every unit were slower (58 us became 61 to 96).
+// for every unit were slower (58 us became 61 to 96), and so were CTAs that take
+// over units which have not started (clusterlaunchcontrol), with the next
+// unit's first keys under way during the join (56 became 63): they leave the
+// SMs together at the end, where the tile kernel could have begun.
 #define PD_WARPS 4
 #define PD_TK 16                // keys of a tile
 #define PD_LAZY 8.0f            // a row is rescaled when its maximum grew by 2^8 or more
