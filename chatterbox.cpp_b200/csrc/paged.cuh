@@ -416,6 +416,11 @@ __device__ __forceinline__ void pg_split2(float x, float y, unsigned & hi, unsig
     hi = *(const unsigned *) &h;
     lo = *(const unsigned *) &l;
 }
+// the same for bf16
+__device__ __forceinline__ void pg_split2_bf16(float x, float y, unsigned & hi, unsigned & lo) {
+    hi = pg_pack2<__nv_bfloat16>(x, y);
+    lo = pg_pack2<__nv_bfloat16>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+}
 // The power of two by which an F32 query row is divided before it is split:
 // it brings the row's largest element to [2^8, 2^9), so that neither part
 // leaves f16's range.  Zero and non-finite rows keep their values.
@@ -455,9 +460,12 @@ __host__ __device__ constexpr int pd_smem(int D) { return PD_WARPS * pd_stages(D
 
 // grid = (splits, n_kv_head, n), clusters of `splits` CTAs, 128 threads
 // MT: tiles of 16 rows; RH: their 8-row halves that hold queries of their own
-// (F32: one, the other has its lo parts; 16-bit: one up to 8 queries, then two)
+// (F32: one; 16-bit: one up to 8 queries, then two).  With one, the other half
+// takes the lo parts: F32's of the queries, and for every type those of the
+// probabilities, which an MMA that runs anyway brings down from a rounding to
+// 11 or 8 bits to one of 22 or 16.
 template <class QT, class CT, int D, int MT, int RH>
-__global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAttn a) {
+__global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) void attn_shared_decode_kernel(PgAttn a) {
     constexpr bool F32 = sizeof(QT) == 4;
     constexpr int RPM = 8 * RH;                    // queries of an M tile
     constexpr int NS = pd_stages(D), KS = D / 16, CH = D / 8;
@@ -699,7 +707,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
 #pragma unroll
                     for (int d = 0; d < D / 8; ++d) {
                         o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c;
-                        if (F32) { o[mt][d][2] *= c; o[mt][d][3] *= c; }
+                        if (RH == 1) { o[mt][d][2] *= c; o[mt][d][3] *= c; }
                     }
                 }
             }
@@ -713,14 +721,15 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
                     l[mt][r] += z[nt][2 * r] + z[nt][2 * r + 1];
                 }
             }
-            if (F32) {
-                pg_split2(z[0][0], z[0][1], p[mt][0], p[mt][1]);
-                pg_split2(z[1][0], z[1][1], p[mt][2], p[mt][3]);
-            } else {
 #pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
+            for (int nt = 0; nt < 2; ++nt) {
+                if (RH == 2) {
                     p[mt][2 * nt] = pg_pack2<CT>(z[nt][0], z[nt][1]);
-                    p[mt][2 * nt + 1] = RH == 2 ? pg_pack2<CT>(z[nt][2 * RH - 2], z[nt][2 * RH - 1]) : 0u;
+                    p[mt][2 * nt + 1] = pg_pack2<CT>(z[nt][2 * RH - 2], z[nt][2 * RH - 1]);
+                } else if (std::is_same<CT, __half>::value) {
+                    pg_split2(z[nt][0], z[nt][1], p[mt][2 * nt], p[mt][2 * nt + 1]);
+                } else {
+                    pg_split2_bf16(z[nt][0], z[nt][1], p[mt][2 * nt], p[mt][2 * nt + 1]);
                 }
             }
         }
@@ -759,7 +768,7 @@ __global__ __launch_bounds__(32 * PD_WARPS) void attn_shared_decode_kernel(PgAtt
             if (q < g) {
 #pragma unroll
                 for (int d = 0; d < D / 8; ++d) {
-                    const float2 v = F32 ? make_float2(o[mt][d][0] + o[mt][d][2], o[mt][d][1] + o[mt][d][3])
+                    const float2 v = RH == 1 ? make_float2(o[mt][d][0] + o[mt][d][2], o[mt][d][1] + o[mt][d][3])
                                          : make_float2(o[mt][d][2 * r], o[mt][d][2 * r + 1]);
                     *(float2 *) (so + (w * g + q) * D + d * 8 + (lane & 3) * 2) = v;
                 }

@@ -444,8 +444,9 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  *
  * Types: q and out F32 with an F16 cache (scores, softmax and sums keep 22
  * bits or more of every factor), or q, out and cache all F16 or all BF16
- * (probabilities are rounded to that type before they meet V, which is less
- * than the output's own rounding; sums stay in F32).  n_head is a multiple
+ * (in prompts, shared prefixes and groups above 8 heads, probabilities are
+ * rounded to that type before they meet V, an error of the size of the
+ * output's own rounding; sums stay in F32).  n_head is a multiple
  * of n_kv_head, at most 16 times it.  scale 0 = 1 / sqrt(head_dim).  q, out
  * and their strides are multiples of 16 bytes.  out may be q (with the same
  * stride).  workspace holds t3b_op_attention_shared_workspace() bytes, 16-byte
