@@ -1097,6 +1097,10 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     if (!s_have || wrong) {                        // the whole cluster: it shares the tile
         if (s_have && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);   // PARTIAL: the decode kernel leaves these requests alone too
         if (warp == MMAW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(TCOLS) : "memory");
+        // The decode kernel let this grid start early: no CTA leaves before it
+        // has ended, or the grid could complete, and what follows it start,
+        // while rows without a prefix are still being written.
+        if (PARTIAL) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     const int cnt = min(ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles

@@ -582,6 +582,58 @@ def test_append_right_behind_a_large_plan(pkg):
     assert torch.equal(pool.cpu().view(2, -1, 64), want)
 
 
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("what", ["no request has a prefix", "every prefix is refused"])
+def test_what_follows_a_shared_call_finds_its_output(pkg, what, graph):
+    """The two-kernel way of a decode call where no row tile has work (all
+    prefix ranges empty, or all prefix lengths refused): a projection queued
+    right behind it, whose kernel may start early, reads what the call wrote."""
+    H, n = 16, 3
+    b = Batch("f32", [3000, 2000, 6000], H, H, 64, 16, [20, 20], [0, 0, 0] if "no" in what else [0, 1, 2], seed=41, share=True)
+    d = b.desc(pkg)
+    assert d.workspace_bytes > 0
+    refused = [] if "no" in what else [0, 1]
+    if refused:
+        b.plen.fill_(16 * b.ptable.shape[1] + 1)
+    L, N = pkg.lib(), 256
+    w = (torch.randn(N, H * 64, generator=torch.Generator().manual_seed(2)) * 0.05).half().numpy()
+    wd = torch.empty(N * L.t3b_op_row_bytes(1, H * 64), dtype=torch.uint8, device="cuda")
+    pkg.check(L.t3b_op_repack(1, w.ctypes.data, N, H * 64, C.c_void_p(wd.data_ptr())))
+    y = torch.zeros(n, N, device="cuda")
+
+    def project():
+        pkg.check(L.t3b_op_gemv(1, C.c_void_p(wd.data_ptr()), N, H * 64, C.c_void_p(b.out_all.data_ptr()), n, None, None, 0.0, None, None, 0,
+                                C.c_void_p(y.data_ptr()), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+
+    def both():
+        pkg.check(L.t3b_op_attention_shared(C.byref(d), C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        project()
+
+    pkg.check(L.t3b_op_attention_shared(C.byref(d), _stream()))
+    torch.cuda.synchronize()
+    project()
+    want = y.clone()
+    torch.cuda.synchronize()
+    run = both
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            both()
+        run = g.replay
+    for _ in range(20):
+        b.out_all.fill_(-7)
+        y.zero_()
+        run()
+        left = b.out_all.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+        assert torch.equal(left, b.out_all)
+    if refused:
+        assert L.t3b_op_check(_stream()) == -5
+        assert (b.out_all[:2] == -7).all()
+    _close(b, skip=refused)
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
