@@ -330,7 +330,9 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 #pragma unroll
         for (int e = 0; e < E; ++e) s = fmaf(qv[e], pg_to(((const CT *) a.k)[off + e]), s);
         s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn), p = mn == -INFINITY ? 0.0f : expf(s - mn);
+        // a NaN score is no maximum (fmaxf passes it over) but has to reach l and o, also before the first finite one
+        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.0f : expf(m - mn);
+        const float p = s == -INFINITY ? 0.0f : expf(s - (mn == -INFINITY ? 0.0f : mn));
         l = l * c + p;
 #pragma unroll
         for (int e = 0; e < E; ++e) o[e] = o[e] * c + p * pg_to(((const CT *) a.v)[off + e]);

@@ -634,6 +634,37 @@ def test_what_follows_a_shared_call_finds_its_output(pkg, what, graph):
     _close(b, skip=refused)
 
 
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("kind,prefix", [("f32", 70), ("bf16", 70), ("f32", 2000), ("f16", 2000)])
+@pytest.mark.parametrize("where", ["q", "first prefix key", "first own key", "a prefix value"])
+def test_nan_reaches_every_row_that_sees_it(pkg, kind, prefix, prompt, share, where):
+    """A NaN in a query or in the K of the first key makes the whole output of
+    the rows and heads that meet it NaN, whatever the order of the keys, and
+    one in a V its element; the other rows and heads stay right."""
+    b = Batch(kind, [100, 30, 40], 6, 2, 64, 16, [prefix], [0, 2], adds=[60, 30, 7] if prompt else None, seed=37, share=share)
+    ref, tol = b.reference()
+    hit = torch.zeros(b.rows, 6, 64, dtype=torch.bool)
+    k, v = (x.view(b.n_pages, b.kv, 16, 64) for x in (b.k, b.v))
+    nan = float("nan")
+    if where == "q":
+        b.q[b.starts[1], 4 * 64 + 9] = nan                        # one row, one head
+        hit[b.starts[1], 4] = True
+    elif where == "first prefix key":
+        k[int(b.ptable[0, 0]), 1, 0, 5] = nan                     # kv head 1: query heads 3, 4 and 5
+        hit[:b.starts[2], 3:] = True
+    elif where == "first own key":
+        k[int(b.table[1, 0]), 1, 0, 5] = nan
+        hit[b.starts[1]:b.starts[2], 3:] = True
+    else:
+        v[int(b.ptable[0, 0]), 1, 3, 5] = nan
+        hit[:b.starts[2], 3:, 5] = True
+    _attend(pkg, b)
+    got = b.out_all[:b.rows].cpu().double()
+    hit = hit.view(b.rows, -1)
+    assert torch.isnan(got[hit]).all()
+    assert ((got - ref).abs() <= tol)[~hit].all()
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
