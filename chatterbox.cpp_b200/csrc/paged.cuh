@@ -961,10 +961,29 @@ __device__ __forceinline__ void pg_mma_ts(unsigned d, unsigned a, unsigned b, un
 // the own keys (PARTIAL: none).
 struct PgTile { int i, px, row0, total, lo, plen, len; };
 
+// whether `cnt` rows from `beg` on are not among the call's `most`
+__device__ __forceinline__ bool pg_range_wrong(int beg, int cnt, int most) { return beg < 0 || cnt < 0 || cnt > most - beg; }
+
+// Reports row ranges that are out of range, wherever they are: a search for a
+// tile ends at the tile's request and sees none behind it.  By T threads.
+template <bool PARTIAL, int T>
+__device__ void pg_check_ranges(const PgAttn & a, int tid) {
+    const int n = PARTIAL ? a.n_prefix : a.n, most = PARTIAL ? a.n : a.rows;
+    const int * start = PARTIAL ? a.prefix_start : a.row_start;
+    bool bad = false;
+#pragma unroll 4
+    for (int x = tid; x < n; x += T) {
+        const int beg = __ldg(start + x);
+        bad |= pg_range_wrong(beg, __ldg(start + x + 1) - beg, most);
+    }
+    if (bad) atomicOr(&g_paged_err, T3B_DEVERR_POS);
+}
+
 // The z-th tile of ROWS rows over all requests (prompt) or prefixes, found by one
 // warp; false past the last one.  Requests whose rows are out of range are
-// passed over.  What the tile needs of its request is loaded beside the
-// starts, and up to 32 prefixes beside those: one trip to memory.
+// passed over (pg_check_ranges reports them).  What the tile needs of its
+// request is loaded beside the starts, and up to 32 prefixes beside those: one
+// trip to memory for every 32 requests up to the tile's.
 template <bool PARTIAL, int ROWS>
 __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
     const int lane = threadIdx.x & 31, n = PARTIAL ? a.n_prefix : a.n;
@@ -981,10 +1000,7 @@ __device__ bool pg_find_tile(const PgAttn & a, int z, PgTile & t) {
         int beg = 0, cnt = 0, ln = 0;
         if (x < n) {
             beg = __ldg(start + x); cnt = __ldg(start + x + 1) - beg; ln = __ldg(lens + x);
-            if (beg < 0 || cnt < 0 || cnt > most - beg) {
-                if (z == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);
-                cnt = 0;
-            }
+            if (pg_range_wrong(beg, cnt, most)) cnt = 0;
         }
         const int mine = (int) (((long long) cnt * a.group + ROWS - 1) / ROWS);
         int inc = mine;
@@ -1069,6 +1085,7 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
         const bool have = pg_find_tile<PARTIAL, ROWS>(a, (int) (gridDim.x / nrank) / a.n_kv_head - 1 - unit / a.n_kv_head, t);
         if (lane == 0) { s_have = have; s_tile = t; s_bad = 0; }
     }
+    if (blockIdx.x == 0 && (warp == 2 || warp == 3)) pg_check_ranges<PARTIAL, 64>(a, tid - 64);   // beside warp 0's search
     if (tid == 32) {
         for (int s = 0; s < R; ++s) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full(s)), "n"(PT_LOADERS) : "memory");

@@ -438,9 +438,10 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  *   row_start[n] on stay as they were.
  *
  * A row with no key at all (or only scores of -infinity) is zero.  A request whose length is negative or
- * past its table, or whose rows exceed its length, and a prefix length past
- * its table leave their rows unwritten and are reported; a page id outside
- * the pool is reported and its keys count as absent.
+ * past its table, whose rows exceed its length or are not among the call's
+ * `rows`, and a prefix length past its table leave their rows unwritten and
+ * are reported (requests and prefixes without rows are not looked at); a page
+ * id outside the pool is reported and its keys count as absent.
  *
  * Types: q and out F32 with an F16 cache (scores, softmax and sums keep 22
  * bits or more of every factor), or q, out and cache all F16 or all BF16

@@ -665,6 +665,45 @@ def test_nan_reaches_every_row_that_sees_it(pkg, kind, prefix, prompt, share, wh
     assert ((got - ref).abs() <= tol)[~hit].all()
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(4, 2, 64), (8, 1, 128)])
+@pytest.mark.parametrize("what", ["past the rows", "all past the rows", "backwards", "below zero"])
+def test_row_ranges_out_of_bounds_are_reported_wherever_they_are(pkg, heads, kv, dim, what):
+    """A bad row range is reported, and the other requests are right, also
+    behind the first requests and behind the last row tile."""
+    n, at = 100, 70
+    adds = [1 + i % 3 for i in range(n)]
+    b = Batch("f16", [5 + a for a in adds], heads, kv, dim, 16, [20], [0, n], adds=adds, seed=38)
+    rows = b.rows
+    if what == "past the rows":                                   # rows that the call does not have: the last 30 requests'
+        rows, skip = b.starts[at], range(at, n)
+    elif what == "all past the rows":
+        rows, skip = 1, range(1, n)
+    elif what == "backwards":                                     # request 70 ends before it begins, 71 has a row of 69's too
+        b.row_start[at + 1] = b.starts[at] - 1
+        skip = [at - 1, at, at + 1]
+    else:
+        b.row_start[0], skip = -2, [0]
+    _attend(pkg, b, rows=rows)
+    assert pkg.lib().t3b_op_check(_stream()) == -5
+    assert "length-out-of-range" in pkg.last_error()
+    _close(b, skip=skip)
+    if what in ("past the rows", "all past the rows", "below zero"):
+        assert all((b.out_all[b.starts[i]:b.starts[i + 1]] == -7).all() for i in skip)
+
+
+def test_prefix_ranges_out_of_bounds_are_reported_wherever_they_are(pkg):
+    """The same for the prefixes of a decode batch: the last of 70 has
+    requests that the call does not have."""
+    G = 70
+    start = list(range(0, 2 * G + 1, 2))
+    b = Batch("f32", [9] * (2 * G), 4, 4, 64, 16, [20] * G, start, seed=39, share=True)
+    b.pstart[G] = 2 * G + 1
+    _attend(pkg, b)
+    assert pkg.lib().t3b_op_check(_stream()) == -5
+    assert "length-out-of-range" in pkg.last_error()
+    _close(b, skip=[2 * G - 2, 2 * G - 1])
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
