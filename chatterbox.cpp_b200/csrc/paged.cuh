@@ -1675,7 +1675,8 @@ PgAttn pg_args(const t3b_shared_attn & a, bool prompt) {
     p.prefix_start = a.prefix_start; p.prefix_len = a.prefix_len; p.prefix_table = a.prefix_table;
     p.n = a.n; p.rows = a.rows; p.n_head = a.n_head; p.n_kv_head = a.cache.n_kv_head; p.group = a.n_head / a.cache.n_kv_head;
     pg_log2(a.cache.page_size, 3, 8, &p.page_log2);
-    p.n_pages = a.cache.n_pages; p.max_blocks = a.max_blocks; p.n_prefix = a.n_prefix; p.prefix_max_blocks = a.prefix_max_blocks;
+    p.n_pages = a.cache.n_pages; p.max_blocks = a.max_blocks; p.n_prefix = a.n_prefix;
+    p.prefix_max_blocks = a.n_prefix > 0 ? a.prefix_max_blocks : 0;   // (not looked at without prefixes)
     p.pass = (double) a.n * a.max_blocks * a.cache.page_size * a.cache.n_kv_head * a.cache.head_dim * 4.0 > 64e6;
     p.part = pg_workspace(a, prompt) ? (float *) a.workspace : nullptr;
     p.scale = a.scale != 0.0f ? a.scale : 1.0f / sqrtf((float) a.cache.head_dim);

@@ -704,6 +704,18 @@ def test_prefix_ranges_out_of_bounds_are_reported_wherever_they_are(pkg):
     _close(b, skip=[2 * G - 2, 2 * G - 1])
 
 
+@pytest.mark.parametrize("prompt", [False, True])
+@pytest.mark.parametrize("room", [-1, -(1 << 31), 1 << 27, (1 << 31) - 1])
+def test_prefix_room_counts_for_nothing_without_prefixes(pkg, prompt, room):
+    b = Batch("f32", [40, 3, 70], 4, 2, 64, 16, adds=[4, 3, 70] if prompt else None, seed=40)
+    d = b.desc(pkg)
+    d.prefix_max_blocks = room
+    f = pkg.lib().t3b_op_attention_shared_prompt if prompt else pkg.lib().t3b_op_attention_shared
+    pkg.check(f(C.byref(d), _stream()))
+    torch.cuda.synchronize()
+    _close(b)
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
