@@ -117,6 +117,9 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(t3b_kv_plan p) {
     pg_plan_rows<4>(p, n, pg_sm[n], lg, r0, pg_sm, start, page);
 }
 
+// who fills in the row maps: nobody (none is wanted), the plan kernel, or kv_plan_rows_kernel
+enum class PgRowMaps { none, here, apart };
+
 // One cluster.  Every CTA scans all requests (a few KB), so all of them know
 // each request's first row, first new page and first returned page and come
 // to the same verdict; the returned pages, the new pages and the rows are
@@ -127,13 +130,13 @@ __global__ __launch_bounds__(256) void kv_plan_rows_kernel(t3b_kv_plan p) {
 // one step and the outputs be the inputs' own buffers.  Bound by latency: a
 // launch, two trips to memory and the scan, 3.9 us for 64 requests (a graph
 // node that does nothing takes 2).
-__global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p, bool rows_here) {
+__global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p, PgRowMaps maps) {
     extern __shared__ int pg_sm[];
     __shared__ unsigned long long red[32][2];
     int * s_len = pg_sm, * s_take = s_len + p.n, * s_back = s_take + p.n, * s_row = s_back + p.n;   // s_row: n + 1
     const int tid = threadIdx.x, T = blockDim.x, n = p.n, P = p.page_size, lg = __ffs(P) - 1;
     unsigned rank, csize;
-    if (!rows_here) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (maps == PgRowMaps::apart) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(csize));
     const long long cap = (long long) p.max_blocks * P;
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(PG_PLAN_T, 1) void kv_plan_kernel(t3b_kv_plan p, bo
             const int i = pg_find(s_take, n, k);
             p.table[(size_t) i * p.max_blocks + ((s_len[i] + P - 1) >> lg) + (k - s_take[i])] = p.free_pages[top - 1 - k];
         }
-    if (rows_here) {
+    if (maps == PgRowMaps::here) {
         auto page = [&](int i, int blk) {
             const int held = (s_len[i] + P - 1) >> lg;
             return blk < held ? p.table[(size_t) i * p.max_blocks + blk] : p.free_pages[top - 1 - (s_take[i] + blk - held)];
@@ -1829,21 +1832,22 @@ int t3b_op_kv_plan(const t3b_kv_plan * p, void * cuda_stream) {
         return T3B_ERR_CUDA;
     }
     // one CTA does for few requests and rows; eight cost 0.3 us more and take a larger step's work apart
-    const bool rows_here = p->rows_cap <= PG_PLAN_ROWS || (!p->row_req && !p->row_pos && !p->slots);
-    const int most = std::max(p->n, p->rows_cap);
+    const int rows = p->row_req || p->row_pos || p->slots ? p->rows_cap : 0;   // that the maps hold
+    const PgRowMaps maps = rows == 0 ? PgRowMaps::none : rows <= PG_PLAN_ROWS ? PgRowMaps::here : PgRowMaps::apart;
+    const int most = std::max(p->n, rows);
     const unsigned threads = most <= 128 ? 128 : most <= 256 ? 256 : PG_PLAN_T;
-    const unsigned c = p->n <= PG_PLAN_T && p->rows_cap <= PG_PLAN_T ? 1 : PG_PLAN_CLUSTER;
+    const unsigned c = p->n <= PG_PLAN_T && rows <= PG_PLAN_T ? 1 : PG_PLAN_CLUSTER;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = c; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3(c); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem;
     cfg.stream = (cudaStream_t) cuda_stream; cfg.attrs = at; cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, *p, rows_here);
-    if (e == cudaSuccess && !rows_here) {
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv_plan_kernel, *p, maps);
+    if (e == cudaSuccess && maps == PgRowMaps::apart) {
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.gridDim = dim3((unsigned) ((p->rows_cap + 1023) / 1024)); cfg.blockDim = dim3(256);
+        cfg.gridDim = dim3((unsigned) ((rows + 1023) / 1024)); cfg.blockDim = dim3(256);
         cfg.dynamicSmemBytes = ((size_t) p->n + 1) * sizeof(int);
         e = cudaLaunchKernelEx(&cfg, kv_plan_rows_kernel, *p);
     }

@@ -147,6 +147,21 @@ def test_plan_without_the_optional_arrays(pkg):
     assert (got["row_req"] == 77).all() and (got["len_out"] == 77).all()
 
 
+def test_plan_without_row_maps_does_not_look_for_rows(pkg):
+    """Without row_req, row_pos and slots no row is mapped: ids of pages that
+    are held already, which only the maps need, are not looked at."""
+    rng = np.random.default_rng(6)
+    ln, add, _, table, free, n_free = _random_step(rng, 40, 16, 6, False)
+    ln[0], add[0], table[0, 0] = 5, 1, -9
+    p = Plan(pkg, ln, add, None, 16, table, free, n_free, int(add.sum()), want=False)
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    pkg.check(pkg.lib().t3b_op_check(_stream()))
+    ref = paged_ref.plan(ln, add, None, 16, table, free, n_free, int(add.sum()))
+    got = p.got()
+    _same({k: got[k] for k in ("table", "free", "n_free", "row_start")},
+          {k: ref[k] for k in ("table", "free", "n_free", "row_start")})
+
+
 BAD_STEPS = {
     "negative length": dict(len={3: -1}), "negative new": dict(add={0: -2}), "negative release": dict(release={2: -7}),
     "past the table": dict(add={1: 97}), "far past the table": dict(add={1: 2 ** 31 - 1}), "release past the table": dict(release={2: 97}, len={2: 0}),
