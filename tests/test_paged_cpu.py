@@ -79,6 +79,31 @@ def test_a_short_workspace_is_refused(pkg):
     assert sizes == sorted(sizes)
 
 
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(8, 4, 64, 0), (16, 1, 128, 1), (6, 2, 128, 0)])
+def test_a_batch_that_shares_a_long_prefix_needs_its_workspace(pkg, heads, kv, dim, dtype):
+    """Where a prefix is computed once for the batch (re-reading it would
+    cost over 48 MB) the workspace holds an own part of head_dim + 4 floats a
+    row and head, and a call without it is refused before anything runs."""
+    L = pkg.lib()
+    kw = dict(n_head=heads, q_stride=heads * dim, out_stride=heads * dim, dtype=dtype, prefix_max_blocks=2000)
+
+    def attn(n, **more):
+        return _attn(pkg, dict(n_kv_head=kv, head_dim=dim), **{**kw, "n": n, "rows": n, **more})
+
+    n = 64
+    need = L.t3b_op_attention_shared_workspace(C.byref(attn(n)))
+    assert (n - 1) * 2000 * 16 * 4 * kv * dim > 48e6
+    assert need == n * heads * (dim + 4) * 4
+    for bad in (dict(workspace=None), dict(workspace=PTR + 4), dict(workspace_bytes=need - 1), dict(workspace_bytes=0)):
+        assert L.t3b_op_attention_shared(C.byref(attn(n, **bad)), None) == -1, bad
+        assert "workspace" in pkg.last_error() and str(need) in pkg.last_error()
+    # pointers are not looked at, and more requests never need less, on both sides of the 48 MB
+    sizes = [L.t3b_op_attention_shared_workspace(C.byref(attn(m, q=None, workspace=None, prefix_max_blocks=200))) for m in (1, 2, 8, 64, 500, 65535)]
+    assert sizes == sorted(sizes) and sizes[0] == 0 and sizes[-1] == 65535 * heads * (dim + 4) * 4
+    # a prompt needs none
+    assert L.t3b_op_attention_shared_workspace(C.byref(attn(n, rows=n + 1))) == 0
+
+
 @pytest.mark.parametrize("bad", [dict(k=None), dict(v=None), dict(slots=None), dict(rows=-1), dict(dtype=30), dict(dtype=8),
                                  dict(stride=255), dict(stride=258), dict(k=PTR + 8), dict(v=PTR + 4)], ids=str)
 def test_bad_appends_are_refused(pkg, bad):
