@@ -356,6 +356,15 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 // S = Q K^T comes out in the layout in which P enters P V, so the softmax
 // stays in registers.  F32 queries take two rows, hi and lo, of 11 bits each
 // (K and V are exact in f16), and so do their probabilities.
+// The tensor cores cut their 32-bit sums off instead of rounding them, always
+// towards zero: one accumulator over 8000 keys shrank F32 outputs by 2.2e-6 and
+// left them 2.5e-6 off (2-norm).  So the MMAs of P V start from zero and each
+// 16-key tile is added with rounding, its hi and lo rows to one sum (3.7e-7 at
+// 64 dimensions, 4.3e-7 at 128); that takes half the registers, and no time
+// (64 CFG streams 59 us both ways, 192 long requests 327 and 326).  Groups
+// above 8 of 16-bit queries, whose outputs are rounded to 11 or 8 bits, keep
+// the MMA's own sum, and round their probabilities to those bits once: both
+// halves of a tile hold queries, and a lo part would take a second MMA.
 //
 // Four warps and 48 (64 dimensions) or 64 KB a CTA let four or three CTAs share
 // an SM, with about 100 KB in flight: 192 requests of 500 to 4000 keys (f16, 8 x
@@ -642,14 +651,16 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
         }
     }
 
-    float o[MT][D / 8][4];
+    float o[MT][D / 8][2 * RH];                    // (RH == 1: hi and lo parts in one sum)
     float m[MT][RH], l[MT][RH];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
         for (int r = 0; r < RH; ++r) { m[mt][r] = -INFINITY; l[mt][r] = 0.0f; }
 #pragma unroll
-        for (int d = 0; d < D / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.0f;
+        for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+            for (int e = 0; e < 2 * RH; ++e) o[mt][d][e] = 0.0f;
     }
     const int lr = lane & 7, mi = lane >> 3;       // ldmatrix: row of matrix mi
     int slot = 0, slot_in = NS - 1;                // stages of tiles x and x + NS - 1
@@ -710,10 +721,7 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
                     const float c = m[mt][r] == -INFINITY ? 0.0f : pg_exp2(m[mt][r] - top[r]);
                     m[mt][r] = top[r]; l[mt][r] *= c;
 #pragma unroll
-                    for (int d = 0; d < D / 8; ++d) {
-                        o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c;
-                        if (RH == 1) { o[mt][d][2] *= c; o[mt][d][3] *= c; }
-                    }
+                    for (int d = 0; d < D / 8; ++d) { o[mt][d][2 * r] *= c; o[mt][d][2 * r + 1] *= c; }
                 }
             }
 #pragma unroll
@@ -745,8 +753,16 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
             pg_ldm4t(b, st + TILE + row * (D * 2) + ((ch ^ lr) << 4));
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                pg_mma<CT>(o[mt][2 * d], p[mt], b[0], b[1]);
-                pg_mma<CT>(o[mt][2 * d + 1], p[mt], b[2], b[3]);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    if constexpr (RH == 2) {
+                        pg_mma<CT>(o[mt][2 * d + y], p[mt], b[2 * y], b[2 * y + 1]);
+                    } else {                       // the tile's sum by itself, then added with rounding
+                        float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        pg_mma<CT>(t, p[mt], b[2 * y], b[2 * y + 1]);
+                        o[mt][2 * d + y][0] += t[0] + t[2]; o[mt][2 * d + y][1] += t[1] + t[3];
+                    }
+                }
             }
         }
         __syncwarp();
@@ -773,9 +789,7 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
             if (q < g) {
 #pragma unroll
                 for (int d = 0; d < D / 8; ++d) {
-                    const float2 v = RH == 1 ? make_float2(o[mt][d][0] + o[mt][d][2], o[mt][d][1] + o[mt][d][3])
-                                         : make_float2(o[mt][d][2 * r], o[mt][d][2 * r + 1]);
-                    *(float2 *) (so + (w * g + q) * D + d * 8 + (lane & 3) * 2) = v;
+                    *(float2 *) (so + (w * g + q) * D + d * 8 + (lane & 3) * 2) = make_float2(o[mt][d][2 * r], o[mt][d][2 * r + 1]);
                 }
                 if ((lane & 3) == 0) { sm[w * g + q] = m[mt][r]; ss[w * g + q] = l[mt][r]; }
             }
@@ -871,9 +885,15 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
 // * O stays in tensor memory and is rescaled only when a row's maximum has
 //   grown by 2^8 since the last time (as in the decode kernel).
 // * F32 queries are two f16 parts, and so are their probabilities: two MMAs
-//   into one accumulator.  The tensor cores' sums are cut off, not rounded, to
-//   32 bits: over 8000 keys in one accumulator that shrank O by 4.4e-6.  So F32
-//   accumulates one key tile at a time, and the softmax threads add the tiles.
+//   into one accumulator, lo first: the tensor cores' sums are cut off, not
+//   rounded, to 32 bits at every step, which costs least while they are small
+//   (8000 keys x 128 dimensions 5.9e-7 off, 2-norm; hi first 1.0e-6).  Over 8000
+//   keys in one accumulator that shrank O by 4.4e-6.  So F32 accumulates one
+//   key tile at a time, and the softmax threads add the tiles.
+// * 16-bit probabilities are rounded to the cache's type once, as they enter P V:
+//   an error of the size of the output's own rounding (2-norm f16 2.9e-4 against
+//   2.1e-4, bf16 2.3e-3 against 1.7e-3), where a lo part would double P V's
+//   MMAs.  The row sum l is of the unrounded ones, in 32 bits.
 // * The keys of a tile of rows may be split over a cluster (few rows, many
 //   keys); its CTAs join their (O, max, sum) over distributed shared memory.
 //
@@ -1346,22 +1366,22 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
         auto qk = [&](int x, int slot) {            // S of tile x = Q K^T
             const unsigned qa = q0 + x * (QTILE >> 4), ka = k0 + slot * (SLOT >> 4);
 #pragma unroll
-            for (int part = 0; part < PARTS; ++part)
+            for (int part = PARTS - 1; part >= 0; --part)      // F32: the small lo parts first, before the sum is large
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const unsigned off = (k >> 2) * (PT_PANEL >> 4) + (k & 3) * 2;
-                    pg_mma_ss(tm + 128 * x, qa + part * (SLOT >> 4) + off, ka + off, ID_QK, part || k ? 1u : 0u, el);
+                    pg_mma_ss(tm + 128 * x, qa + part * (SLOT >> 4) + off, ka + off, ID_QK, part < PARTS - 1 || k ? 1u : 0u, el);
                 }
             pg_commit(s_full(x), el);
         };
         auto pv = [&](int x, int slot, unsigned acc, int half) {   // O of tile x += P V over half of the tile's keys
             const unsigned va = v0 + slot * (SLOT >> 4);
 #pragma unroll
-            for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
+            for (int part = PARTS - 1; part >= 0; --part)
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part)
+                for (int k = half * PT_BN / 32; k < (half + 1) * PT_BN / 32; ++k)
                     pg_mma_ts(tm + 128 * NT + D * x, tm + 128 * x + (F32 ? 32 * (k >> 1) + 16 * part + 8 * (k & 1) : 8 * k), va + k * 128,
-                              ID_PV, half == 0 && k == 0 && part == 0 ? acc : 1u, el);
+                              ID_PV, half == 0 && k == 0 && part == PARTS - 1 ? acc : 1u, el);
         };
         bool ok = tf_wait(q_full, 0u);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

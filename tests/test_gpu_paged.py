@@ -731,6 +731,37 @@ def test_prefix_room_counts_for_nothing_without_prefixes(pkg, prompt, room):
     _close(b)
 
 
+@pytest.mark.parametrize("mode", ["prompt", "shared", "own"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_f32_over_8000_keys_of_one_cta(pkg, mode, dim):
+    """F32 outputs stay within 1e-6 of 64 bits (2-norm) where one CTA takes
+    all of 8000 keys: 5 row tiles of 16 heads are more than half of 148 SMs
+    and 40 requests of 16 heads more than four times as many, so nothing is
+    split.  What is off in 32 bits: weights of 22 bits, 2^-22 / sqrt(3) =
+    1.4e-7; exponents of up to 2^3 held to 2^-22, 2e-7; scores, whose sum of
+    dim / 16 steps loses up to 2^-24 of itself at each, 5e-7 at 128 dimensions
+    times a weighted spread of about 1 between the scores; at most 500
+    roundings of O, sqrt(500) 2^-25 = 7e-7 where they all met its final size
+    and half of that as it grows.  Squares added: 7e-7.  One running sum of
+    the tensor cores, which is cut off at each step, comes to 2.5e-6 and more."""
+    G, H = 5, 16
+    adds = [3] * G if mode == "prompt" else None
+    per = 1 if mode == "prompt" else 2
+    if mode == "own":
+        b = Batch("f32", [8000] * 40, H, H, dim, 64, seed=42)
+    else:
+        b = Batch("f32", [3] * (G * per), H, H, dim, 64, [8000] * G, [per * i for i in range(G + 1)], adds=adds, seed=42, share=mode == "shared")
+    d = _attend(pkg, b)
+    assert (d.workspace_bytes > 0) == (mode == "shared")
+    _close(b)
+    ref, _ = b.reference()
+    got = b.out_all[:b.rows].cpu().double()
+    assert (got - ref).norm() / ref.norm() < 1e-6
+    for i in range(len(b.lens)):                                  # each request by itself too
+        rows = slice(b.starts[i], b.starts[i + 1])
+        assert (got - ref)[rows].norm() / ref[rows].norm() < 1e-6
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
