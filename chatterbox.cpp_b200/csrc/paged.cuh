@@ -360,9 +360,11 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 // towards zero: one accumulator over 8000 keys shrank F32 outputs by 2.2e-6 and
 // left them 2.5e-6 off (2-norm).  So the MMAs of P V start from zero and each
 // 16-key tile is added with rounding, its hi and lo rows to one sum (3.7e-7 at
-// 64 dimensions, 4.3e-7 at 128); that takes half the registers, and no time
-// (64 CFG streams 59 us both ways, 192 long requests 327 and 326).  Groups
-// above 8 of 16-bit queries, whose outputs are rounded to 11 or 8 bits, keep
+// 64 dimensions, 4.3e-7 at 128).  That takes half the registers (16 bits x 128
+// dimensions spilled 44 bytes before) and little time: 64 CFG streams 56.0 us
+// before and 56.1 since, 256 short answers 53.8 and 53.2, 192 long requests
+// 296.3 and 296.2, F32 groups of 16 heads 43.4 and 44.2.  Groups above 8 of
+// 16-bit queries, whose outputs are rounded to 11 or 8 bits, keep
 // the MMA's own sum, and round their probabilities to those bits once: both
 // halves of a tile hold queries, and a lo part would take a second MMA.
 //
@@ -1139,10 +1141,12 @@ __global__ __launch_bounds__(pt_threads(NT), 3 - NT) void attn_shared_tile_kerne
     if (!s_have || wrong) {                        // the whole cluster: it shares the tile
         if (s_have && tid == 0) atomicOr(&g_paged_err, T3B_DEVERR_POS);   // PARTIAL: the decode kernel leaves these requests alone too
         if (warp == MMAW) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(TCOLS) : "memory");
-        // The decode kernel let this grid start early: no CTA leaves before it
-        // has ended, or the grid could complete, and what follows it start,
-        // while rows without a prefix are still being written.
-        if (PARTIAL) asm volatile("griddepcontrol.wait;" ::: "memory");
+        // The decode kernel let this grid start early, and what follows must find
+        // rows without a prefix written: the grid cannot complete before the
+        // decode kernel while one CTA waits for it, here or in the epilogue.
+        // That is the last to start, tile 0's; the surplus ones start first and
+        // would hold SMs that tiles need (192 long requests 296 us became 301).
+        if (PARTIAL && unit == (int) (gridDim.x / nrank) - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     const int cnt = min(ROWS, t.total - t.lo), nt = cnt > 128 ? 2 : 1;   // rows, 128-row tiles
