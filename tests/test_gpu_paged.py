@@ -762,6 +762,19 @@ def test_f32_over_8000_keys_of_one_cta(pkg, mode, dim):
         assert (got - ref)[rows].norm() / ref[rows].norm() < 1e-6
 
 
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("kind,heads,kv,dim", [("f16", 8, 2, 128), ("bf16", 8, 2, 128), ("bf16", 16, 1, 64), ("f16", 32, 2, 128)])
+def test_repeated_16_bit_calls_give_the_same_bits(pkg, kind, heads, kv, dim, prompt, share):
+    b = Batch(kind, [40, 900, 7, 333] * 6, heads, kv, dim, 16, [4001], [0, 24], adds=[40, 260, 7, 100] * 6 if prompt else None, seed=43, share=share)
+    _attend(pkg, b)
+    first = b.out_all.clone()
+    _close(b)
+    for _ in range(5):
+        b.out_all.fill_(-7)
+        _attend(pkg, b)
+        assert torch.equal(b.out_all, first)
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
