@@ -333,7 +333,11 @@ int t3b_op_attention_noalloc(const float * q_dev, const void * k_dev, const void
  * One step of a serving loop: t3b_op_kv_plan (pages, slots and positions of
  * the new tokens), then for each layer t3b_op_kv_append and
  * t3b_op_attention_shared (one token per request) or
- * t3b_op_attention_shared_prompt (several).  All of it runs on the caller's
+ * t3b_op_attention_shared_prompt (several).  The plan, the append and the
+ * prompt form take a step's rows in one compact order, where a request
+ * without a new token has none; the decode form has row i for request i, so
+ * that in a step with such requests K and V are gathered through row_req (or
+ * the prompt form is used).  All of it runs on the caller's
  * stream without a host synchronisation or an allocation, so a step can be
  * captured into a CUDA graph; the structs are read during the call only.
  * Pointers are device pointers of the current device unless noted.  Errors

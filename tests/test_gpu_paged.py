@@ -882,3 +882,80 @@ def test_a_serving_loop_matches_dense_attention(pkg, graph, share):
         assert (out[:total] - want).abs().max() <= 1e-5 * want.abs().max()     # the bound of each against 64 bits
         assert (out[total:] == -7).all()
         lens = lens + a
+
+
+@pytest.mark.parametrize("form", ["decode", "prompt"])
+def test_a_serving_loop_with_idle_slots(pkg, form):
+    """Steps in which some slots get no token: the plan's rows are compact
+    (row r belongs to slot row_req[r]), the decode form's are by slot.  The
+    decode form takes q by slot, and its K/V rows are gathered through row_req
+    for the append; the prompt form takes all of them in the plan's order,
+    prompts of admitted requests among them.  Every row against 64 bits."""
+    L = pkg.lib()
+    H, D, page, n, width, cap, P = 4, 64, 8, 7, 6, 64, 21
+    rng = np.random.default_rng(19)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n_pages, pre = 50, blocks(P, page)
+    pool = torch.full((2, n_pages, H, page, D), float("nan"), dtype=torch.float16, device="cuda")
+    prefix = torch.randn(2, P, H, D, generator=g, device="cuda").half()
+    for t in range(P):
+        pool[:, t // page, :, t % page] = prefix[:, t]
+    held = [prefix.new_zeros(2, 0, H, D) for _ in range(n)]       # the own K and V of each slot
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    ln, add, rel, table, row_start = z(n), z(n), z(n), z(n, width), z(n + 1)
+    req, pos, slots = z(cap), z(cap), z(cap)
+    free, n_free = torch.arange(pre, n_pages, dtype=torch.int32, device="cuda"), _i32([n_pages - pre])
+    ptable, plen, pstart = torch.arange(pre, dtype=torch.int32, device="cuda"), _i32([P]), _i32([0, n])
+    q, k, v, out = (torch.zeros(cap, H * D, device="cuda") for _ in range(4))
+    p = lambda t: t.data_ptr()  # noqa: E731
+    dplan = pkg.KvPlan(n=n, page_size=page, max_blocks=width, rows_cap=cap, len=p(ln), add=p(add), release=p(rel), free_pages=p(free),
+                       free_cap=free.numel(), n_free=p(n_free), n_free_out=p(n_free), table=p(table), row_start=p(row_start),
+                       row_req=p(req), row_pos=p(pos), slots=p(slots), len_out=p(ln))
+    cache = pkg.PagedKv(k=p(pool[0]), v=p(pool[1]), dtype=1, n_pages=n_pages, n_kv_head=H, page_size=page, head_dim=D)
+    app = pkg.KvAppend(cache=cache, k=p(k), v=p(v), stride=H * D, slots=p(slots), dtype=0, rows=cap)
+    at = pkg.SharedAttn(cache=cache, q=p(q), out=p(out), q_stride=H * D, out_stride=H * D, len=p(ln), table=p(table), prefix_start=p(pstart),
+                        prefix_len=p(plen), prefix_table=p(ptable), dtype=0, n_head=H, n=n, rows=n, max_blocks=width, n_prefix=1,
+                        prefix_max_blocks=pre)
+    if form == "prompt":
+        at.row_start, at.rows = p(row_start), cap
+    lens = np.zeros(n, int)
+    for it in range(30):
+        a, r = (rng.random(n) < 0.6).astype(int), np.zeros(n, int)    # some slots idle in every step
+        gone = (lens > 0) & (rng.random(n) < 0.15)
+        r[gone], lens[gone] = lens[gone], 0
+        if form == "prompt":
+            a = np.where((lens == 0) & (a > 0), rng.integers(1, 9, n), a)
+        a[gone & (rng.random(n) < 0.5)] = 0
+        a = np.minimum(a, width * page - lens)
+        for i in np.nonzero(gone)[0]:
+            held[i] = held[i][:, :0]
+        ln.copy_(_i32(lens)); add.copy_(_i32(a)); rel.copy_(_i32(r))
+        starts, total = np.cumsum(np.r_[0, a]), int(a.sum())
+        x = torch.randn(3, n if form == "decode" else cap, H * D, generator=g, device="cuda")   # what the model's QKV step gives
+        out.fill_(-7.0)
+        pkg.check(L.t3b_op_kv_plan(C.byref(dplan), _stream()))
+        q[:x.shape[1]] = x[0]
+        if form == "decode":
+            rows = req.clamp(min=0).long()
+            k.copy_(x[1][rows]); v.copy_(x[2][rows])
+        else:
+            k.copy_(x[1]); v.copy_(x[2])
+        pkg.check(L.t3b_op_kv_append(C.byref(app), _stream()))
+        pkg.check((L.t3b_op_attention_shared if form == "decode" else L.t3b_op_attention_shared_prompt)(C.byref(at), _stream()))
+        pkg.check(L.t3b_op_check(_stream()))
+        assert row_start.tolist() == starts.tolist() and (req[total:] == -1).all()
+        for i in range(n):
+            own = slice(i, i + a[i]) if form == "decode" else slice(starts[i], starts[i] + a[i])
+            new = x[1:, own].half().view(2, -1, H, D)
+            held[i] = torch.cat([held[i], new], 1)
+            for t in range(a[i]):
+                kk, vv = torch.cat([prefix, held[i][:, :lens[i] + t + 1]], 1).double()
+                qq = x[0, own.start + t].double().view(H, D)
+                w = torch.softmax(torch.einsum("hd,khd->hk", qq, kk) / 8, -1)
+                want = torch.einsum("hk,khd->hd", w, vv).reshape(-1)
+                # 32-bit results: 2^-18 of the largest value, which is above 64 roundings
+                assert (out[own.start + t].double() - want).abs().max() <= 2.0 ** -18 * vv.abs().max(), (it, i, t)
+        lens = lens + a
+        if form == "prompt":
+            assert (out[total:] == -7).all()
+    assert lens.max() > page                                      # requests grew over several pages
