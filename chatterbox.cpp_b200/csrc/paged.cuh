@@ -251,8 +251,8 @@ __device__ __forceinline__ uint4 pg_pack8(const S * src) {
 
 // A thread moves eight elements of K and the same eight of V, U times over.
 // Bound by HBM.  U = 2 puts both pieces' loads in flight before the first
-// store: 20001 rows of 8 x 128 bf16 26.0 us (6.3 TB/s, 0.97 of the copy rate)
-// against 26.7 with one; a call that does not fill the GPU twice keeps one
+// store: 20001 rows of 8 x 128 bf16 26.0 to 26.4 us (6.2 to 6.3 TB/s, 0.95 to
+// 0.97 of the copy rate) against 26.7 with one; a call that does not fill the GPU twice keeps one
 // (128 rows of 16 x 64 f32: 2.1 us against 2.5).
 template <class S, class T, int U>
 __global__ __launch_bounds__(256) void kv_append_kernel(PgAppendArgs a) {
@@ -315,6 +315,9 @@ __device__ __forceinline__ int pg_prefix_of(const PgAttn & a, int i) {
 // elements x * D / 32 .. of the output.  The tiled prompt kernel comes here
 // for rows whose output is not finite: a NaN or infinity in the V of a later
 // token that the row does not see meets a probability of zero in its tile.
+// Rows that do see it come here too.  That is dear, about 1.4 us a key and warp:
+// one NaN in the V of a shared prefix takes 8 chunks of 300 to 2000 tokens from
+// 0.34 to 56 ms and 16 text prompts from 24 us to 4.4 ms.
 template <class QT, class CT, int D>
 __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, int px, int plen, int own, int kvh, float (&o)[D / 32]) {
     constexpr int E = D / 32;
@@ -370,8 +373,9 @@ __device__ __noinline__ void pg_row_slow(const PgAttn & a, const QT * q, int i, 
 //
 // Four warps and 48 (64 dimensions) or 64 KB a CTA let four or three CTAs share
 // an SM, with about 100 KB in flight: 192 requests of 500 to 4000 keys (f16, 8 x
-// 128, prefix apart) run at 6.4 TB/s, 0.98 of the copy rate; 128 of 88 to
-// 1088 (f32, 16 x 64) at 5.6, where a quarter of a CTA's 12 us goes to its
+// 128, prefix apart) run at 6.4 TB/s, 0.98 of the copy rate, in a short run and
+// at 5.8 in a long one, under the power cap; 128 of 88 to 1088 (f32, 16 x 64) at
+// 5.6 (5.2 with the call's cost), where a quarter of a CTA's 12 us goes to its
 // first loads and its last join.  Two warps a CTA, deeper rings and a cluster
 // for every unit were slower (58 us became 61 to 96), and so were CTAs that take
 // over units which have not started (clusterlaunchcontrol), with the next
@@ -868,8 +872,9 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
 // A step of 256 x 128 (bf16, 128 dimensions) takes 3600 cycles: 32 MMAs of about
 // 94 cycles (64 if shared memory fed them without a pause: an MMA of Q K^T reads
 // 8 KB) and a softmax of 2500 per tile, half of it beside the other tile's.  Eight
-// chunks of 300 to 2000 tokens (32 heads over 8) come to 865 TFLOP/s, 0.52 of
-// the library GEMM's.  Measured and left: half of the exponentials as a
+// chunks of 300 to 2000 tokens (32 heads over 8) come to 860 TFLOP/s, 0.52 of
+// the library GEMM's, in a short run and to 740 in a long one, 0.53 of what the
+// GEMM keeps up under the power cap.  Measured and left: half of the exponentials as a
 // polynomial on the FMA pipes (336 us became 366), P V and Q K^T interleaved by
 // halves (339), output rows straight from registers (347).
 //
@@ -891,7 +896,8 @@ __global__ __launch_bounds__(32 * PD_WARPS, MT == 1 ? (D == 64 ? 4 : 3) : 1) voi
 //   rounded, to 32 bits at every step, which costs least while they are small
 //   (8000 keys x 128 dimensions 5.9e-7 off, 2-norm; hi first 1.0e-6).  Over 8000
 //   keys in one accumulator that shrank O by 4.4e-6.  So F32 accumulates one
-//   key tile at a time, and the softmax threads add the tiles.
+//   key tile at a time, and the softmax threads add the tiles; 16-bit outputs,
+//   which are rounded by up to 2^-12 or 2^-9 in the end, keep the one sum.
 // * 16-bit probabilities are rounded to the cache's type once, as they enter P V:
 //   an error of the size of the output's own rounding (2-norm f16 2.9e-4 against
 //   2.1e-4, bf16 2.3e-3 against 1.7e-3), where a lo part would double P V's
@@ -1679,7 +1685,9 @@ const char * pg_attn_wrong(const t3b_shared_attn & a, bool prompt, bool pointers
 
 // Whether a decode call computes its prefixes' attention once for the batch
 // (the tile kernel after the decode kernel) or lets every request read its
-// prefix through L2.  The tile kernel costs 6 to 8 us; what it saves is the
+// prefix through L2.  The host has no lengths, so this and the other rules of a
+// launch (splits, what passes through L2) go by the room in the tables; the
+// figures are of tables as wide as their longest request.  The tile kernel costs 6 to 8 us; what it saves is the
 // prefix's K and V for all requests but one, at 5 to 8 TB/s.  Measured with own
 // lengths around 300, us without / with it: 16 x 376 keys (25 MB, f32 x 64
 // dimensions) 14 / 17, 32 x 376 (49 MB) 21 / 25 and (bf16, 8 x 128) 27 / 24,

@@ -430,7 +430,7 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  * keys in the pages of prefix_table[p] and then their own: key j of request
  * i is row j % page_size of page table[i][j / page_size].  Requests outside
  * every range have no prefix; n_prefix 0 needs no prefix pointers.  Table
- * entries past a length are not read.  Query head h reads K/V head h *
+ * entries past a length may hold anything (some are loaded, none is used).  Query head h reads K/V head h *
  * n_kv_head / n_head.  out = softmax(scale * q.K) V, rounded once.
  *
  *   t3b_op_attention_shared: q and out have one row per request (rows = n,
@@ -441,11 +441,17 @@ int t3b_op_kv_append(const t3b_kv_append * a, void * cuda_stream);
  *   AFTER the append.  rows bounds row_start[n]; rows of out from
  *   row_start[n] on stay as they were.
  *
+ * A NaN or infinity in a key or value reaches only rows that see it; an
+ * infinity in a V may come out as a NaN.  Prompt rows with one are slow: they
+ * are worked out again key by key.
  * A row with no key at all (or only scores of -infinity) is zero.  A request whose length is negative or
  * past its table, whose rows exceed its length or are not among the call's
  * `rows`, and a prefix length past its table leave their rows unwritten and
  * are reported (requests and prefixes without rows are not looked at); a page
  * id outside the pool is reported and its keys count as absent.
+ * How a call is split over the GPU goes by max_blocks and prefix_max_blocks,
+ * for which the host needs no lengths: tables much wider than their requests
+ * cost some speed.
  *
  * Types: q and out F32 with an F16 cache (scores, softmax and sums keep 22
  * bits or more of every factor), or q, out and cache all F16 or all BF16
