@@ -775,6 +775,68 @@ def test_repeated_16_bit_calls_give_the_same_bits(pkg, kind, heads, kv, dim, pro
         assert torch.equal(b.out_all, first)
 
 
+@pytest.mark.parametrize("prompt,share", [(False, False), (False, True), (True, False)])
+@pytest.mark.parametrize("kind,heads,kv,dim", [("f32", 4, 4, 64), ("bf16", 8, 2, 128)])
+def test_k_and_v_of_two_layers_in_one_page(pkg, kind, heads, kv, dim, prompt, share):
+    """K and V (and another layer's) side by side in each page, by page_stride;
+    the append writes there too, and nowhere else."""
+    page = 16
+    lens = [40, 3, 17, 200]
+    b = Batch(kind, lens, heads, kv, dim, page, [150], [0, 3], adds=[40, 2, 1, 60] if prompt else None, seed=44, share=share)
+    dense = kv * page * dim
+    pool = torch.full((b.n_pages, 2, 2, dense), float("nan"), dtype=b.k.dtype, device="cuda")    # [page][layer][K, V]
+    pool[:, 1, 0], pool[:, 1, 1] = b.k.view(b.n_pages, dense), b.v.view(b.n_pages, dense)
+    b.stride, b.k, b.v = 4 * dense, pool[0, 1, 0], pool[0, 1, 1]
+    _attend(pkg, b)
+    _close(b)
+    if not prompt and not share:
+        before = pool.clone()
+        new = torch.randn(2, 4, kv * dim, device="cuda")
+        slots = _i32([int(b.table[i, (n - 1) // page]) * page + (n - 1) % page for i, n in enumerate(lens)])
+        c = b.desc(pkg).cache
+        a = pkg.KvAppend(cache=c, k=new[0].data_ptr(), v=new[1].data_ptr(), stride=kv * dim, slots=slots.data_ptr(), dtype=0, rows=4)
+        pkg.check(pkg.lib().t3b_op_kv_append(C.byref(a), _stream()))
+        view = before.view(b.n_pages, 2, 2, kv, page, dim)
+        for r, s in enumerate(slots.tolist()):
+            for x in range(2):
+                view[s // page, 1, x, :, s % page] = new[x, r].to(pool.dtype).view(kv, dim)
+        assert torch.equal(pool.view(torch.int16), before.view(torch.int16))
+
+
+@pytest.mark.parametrize("mode", ["decode", "shared", "prompt"])
+@pytest.mark.parametrize("kind,heads,kv,dim,page", [("f32", 4, 4, 64, 8), ("f16", 8, 2, 128, 32), ("bf16", 32, 2, 128, 16), ("f32", 3, 1, 128, 64)])
+def test_tables_much_wider_than_the_lengths(pkg, mode, kind, heads, kv, dim, page):
+    """Tables with room for thousands of keys and few in them: clusters of
+    which most CTAs have no key."""
+    lens = [1, 0, page, 130, 5]
+    b = Batch(kind, lens, heads, kv, dim, page, [40, 3], [0, 2, 4], adds=[1, 0, page - 1, 130, 2] if mode == "prompt" else None, seed=45)
+    wide = torch.full((len(lens), 6000 // page), 1 << 28, dtype=torch.int32, device="cuda")
+    b.table = torch.cat([b.table, wide], 1).contiguous()
+    room = 50_000_000 // (4 * kv * dim * page * 3) + 1 if mode == "shared" else 3000 // page if mode == "prompt" else 1000 // page
+    b.ptable = torch.cat([b.ptable, torch.full((2, room), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
+    d = _attend(pkg, b)
+    assert (d.workspace_bytes > 0) == (mode == "shared")
+    _close(b)
+
+
+@pytest.mark.parametrize("which", [("row_req", "row_pos", "slots"), ("slots",), ("row_pos",), ("row_req", "slots")])
+@pytest.mark.parametrize("n,page,width", [(50, 16, 12), (900, 16, 12)])
+def test_plan_with_some_row_maps_that_are_not_16_byte_aligned(pkg, which, n, page, width):
+    rng = np.random.default_rng(n)
+    ln, add, release, table, free, n_free = _random_step(rng, n, page, width, True)
+    cap = int(add.sum()) + 3
+    ref = paged_ref.plan(ln, add, release, page, table, free, n_free, cap)
+    p = Plan(pkg, ln, add, release, page, table, free, n_free, cap)
+    for k in ("row_req", "row_pos", "slots"):
+        p.out[k] = torch.full((cap + 4,), 77, dtype=torch.int32, device="cuda")
+        setattr(p.d, k, p.out[k].data_ptr() + 4 if k in which else None)
+    pkg.check(pkg.lib().t3b_op_kv_plan(C.byref(p.d), _stream()))
+    for k in ("row_req", "row_pos", "slots"):
+        got = p.out[k].cpu().numpy()
+        assert got[0] == 77 and (got[cap + 1:] == 77).all()
+        assert np.array_equal(got[1:cap + 1], ref[k]) if k in which else (got == 77).all(), k
+
+
 # --------------------------------------------------------------------------
 # the operators together
 # --------------------------------------------------------------------------
